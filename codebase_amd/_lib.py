@@ -75,6 +75,33 @@ class RetStatsStruct(ctypes.Structure):
                 ("exchange", c_void_p), ("exchange_ctx", c_void_p), ("moments", c_void_p)]
 
 
+class SsmShape(ctypes.Structure):
+    _fields_ = [("n_agents", c_int32), ("steps", c_int32), ("batch", c_int32), ("channels", c_int32), ("state", c_int32), ("groups", c_int32),
+                ("dtype", c_int32), ("n_networks", c_int32), ("net_of", c_int32 * 16)]
+
+
+class SsmSeq(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("agent_stride", c_int64), ("step_stride", c_int64), ("row_stride", c_int64)]
+
+
+class SsmConvArgs(ctypes.Structure):
+    _fields_ = [("x", SsmSeq), ("dy", SsmSeq), ("weight", c_void_p), ("bias", c_void_p), ("silu", c_int32), ("state", c_void_p),
+                ("reset", c_void_p), ("lengths", c_void_p), ("y", c_void_p), ("state_out", c_void_p), ("dstate_out", c_void_p), ("dx", c_void_p),
+                ("dstate", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p)]
+
+
+class SsmScanArgs(ctypes.Structure):
+    _fields_ = [("x", SsmSeq), ("delta", SsmSeq), ("B", SsmSeq), ("C", SsmSeq), ("z", SsmSeq), ("dy", SsmSeq),
+                ("A", c_void_p), ("D", c_void_p), ("delta_bias", c_void_p), ("softplus", c_int32), ("h_in", c_void_p), ("reset", c_void_p),
+                ("lengths", c_void_p), ("y", c_void_p), ("h_out", c_void_p), ("record", c_void_p), ("dh_out", c_void_p), ("dx", c_void_p),
+                ("ddelta", c_void_p), ("dB", c_void_p), ("dC", c_void_p), ("dz", c_void_p), ("dA", c_void_p), ("dD", c_void_p),
+                ("ddelta_bias", c_void_p), ("dh_in", c_void_p)]
+
+
+class TensorStruct(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("out", c_void_p), ("n", c_int64), ("dtype", c_int32)]
+
+
 class IdqnLearner(ctypes.Structure):
     _fields_ = [("net", NetShape), ("rs", ReplayShape), ("rb", ReplayBuffers),
                 ("params", c_void_p), ("target", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p),
@@ -244,6 +271,17 @@ PROTOTYPES = {
                                                 c_void_p, c_void_p, c_void_p]),
     "marlhip_idqn_update_n_split16": (c_int32, [POINTER(IdqnLearner), c_int32, c_int32, c_uint64, c_uint32, POINTER(c_int64),
                                                 POINTER(c_int64), POINTER(c_int64), c_void_p]),
+    "marlhip_ssm_conv": (c_int32, [POINTER(SsmShape), POINTER(SsmConvArgs), c_void_p]),
+    "marlhip_ssm_conv_grad_workspace_bytes": (c_int64, [POINTER(SsmShape)]),
+    "marlhip_ssm_conv_grad": (c_int32, [POINTER(SsmShape), POINTER(SsmConvArgs), c_void_p, c_int64, c_void_p]),
+    "marlhip_ssm_scan_record_floats": (c_int64, [POINTER(SsmShape)]),
+    "marlhip_ssm_scan_workspace_bytes": (c_int64, [POINTER(SsmShape)]),
+    "marlhip_ssm_scan": (c_int32, [POINTER(SsmShape), POINTER(SsmScanArgs), c_void_p, c_int64, c_void_p]),
+    "marlhip_ssm_scan_grad_workspace_bytes": (c_int64, [POINTER(SsmShape)]),
+    "marlhip_ssm_scan_grad": (c_int32, [POINTER(SsmShape), POINTER(SsmScanArgs), c_void_p, c_int64, c_void_p]),
+    "marlhip_grad_norm_workspace_bytes": (c_int64, [POINTER(TensorStruct), c_int32]),
+    "marlhip_grad_norm": (c_int32, [POINTER(TensorStruct), c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
+    "marlhip_clip_grad_norm": (c_int32, [POINTER(TensorStruct), c_int32, c_float, c_void_p, c_void_p, c_int64, c_void_p]),
     "marlhip_timing_enable": (c_int32, [c_int32]),
     "marlhip_timing_read": (c_int32, [c_int32, POINTER(c_int64), POINTER(c_double)]),
     "marlhip_idqn_collect": (c_int32, [POINTER(LbfConfig), POINTER(NetShape), c_void_p, c_float, c_uint32,

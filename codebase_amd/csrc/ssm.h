@@ -1,0 +1,184 @@
+// Shared pieces of the state space sequence operators (ssm_scan.hip, ssm_conv.hip): element types, argument checks, wave helpers.
+//
+// Sequences are [agent][step][row][channel], channels contiguous, any stride elsewhere (marlhip_ssm_seq).  Consecutive lanes own
+// consecutive channels, so every access along the sequence is a coalesced row; the carried state is [agent][row][state][channel] and the
+// weights are [network][..][channel] for the same reason.
+#pragma once
+#include "common.h"
+
+namespace marl {
+
+constexpr int SSM_MAX_STATE = 32;  // states per channel the scan keeps in registers
+constexpr int SSM_MAX_WIDTH = 8;   // taps of the short convolution
+
+template <class T>
+__device__ __forceinline__ float up(T v) { return static_cast<float>(v); }
+// one rounding to the nearest value of T, ties to even (the conversion instructions' own mode)
+template <class T>
+__device__ __forceinline__ T down(float v) { return static_cast<T>(v); }
+
+struct SsmSeq {
+    const void* data;
+    int64_t sp, st, sb;  // elements between agents, steps, rows
+};
+
+inline SsmSeq ssm_seq(const marlhip_ssm_seq& s) { return SsmSeq{s.data, s.agent_stride, s.step_stride, s.row_stride}; }
+
+template <class T>
+__device__ __forceinline__ const T* seq_at(const SsmSeq& s, int p, int b) {
+    return static_cast<const T*>(s.data) + p * s.sp + b * s.sb;
+}
+
+// One row of a wave through a buffer descriptor: the base is uniform, `bytes` of it exist.  Lanes behind them load 0 and store nothing, and
+// with bytes = 0 a whole row is skipped - no predicate registers, no per-lane 64-bit addresses.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+template <class T>
+__device__ __forceinline__ float row_load(const T* base, int bytes, int voff) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(row_rsrc(base, bytes), voff, 0, 0));
+    else return up(__builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(row_rsrc(base, bytes), voff, 0, 0)));
+}
+template <class T>
+__device__ __forceinline__ void row_store(float v, T* base, int bytes, int voff) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), row_rsrc(base, bytes), voff, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, down<T>(v)), row_rsrc(base, bytes), voff, 0, 0);
+}
+
+struct SsmDims {
+    int P, S, B, C, N, G;
+    int8_t net[16];  // agent -> network
+    int M;           // networks
+};
+
+inline SsmDims ssm_dims(const marlhip_ssm_shape* s) {
+    SsmDims d;
+    d.P = s->n_agents; d.S = s->steps; d.B = s->batch; d.C = s->channels; d.N = s->state; d.G = s->groups;
+    d.M = s->n_networks > 0 ? s->n_networks : s->n_agents;
+    for (int i = 0; i < 16; ++i) d.net[i] = (int8_t)(s->n_networks > 0 ? (i < s->n_agents ? s->net_of[i] : 0) : i);
+    return d;
+}
+
+inline int ssm_validate(const marlhip_ssm_shape* s, const char* what) {
+    MARL_REQUIRE(s != nullptr, "%s: shape is NULL", what);
+    MARL_REQUIRE(s->n_agents >= 1 && s->n_agents <= 16, "%s: %d agents (1..16 supported)", what, s->n_agents);
+    MARL_REQUIRE(s->steps >= 0 && s->batch >= 0 && s->channels >= 1, "%s: steps %d, batch %d, channels %d", what, s->steps, s->batch, s->channels);
+    MARL_REQUIRE(s->steps <= (1 << 30) && s->batch <= (1 << 26) && s->channels <= (1 << 20), "%s: steps %d, batch %d, channels %d are too many", what,
+                 s->steps, s->batch, s->channels);
+    MARL_REQUIRE(s->dtype >= 0 && s->dtype <= 2, "%s: dtype %d (0 f32, 1 bf16, 2 f16)", what, s->dtype);
+    if (s->n_networks > 0) {
+        MARL_REQUIRE(s->n_networks <= s->n_agents, "%s: %d networks for %d agents", what, s->n_networks, s->n_agents);
+        for (int i = 0; i < s->n_agents; ++i)
+            MARL_REQUIRE(s->net_of[i] >= 0 && s->net_of[i] < s->n_networks, "%s: net_of[%d] = %d out of range", what, i, s->net_of[i]);
+    }
+    return 0;
+}
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// rows of a padded batch: steps of row b that belong to its sequence
+__device__ __forceinline__ int seq_len(const int32_t* lengths, int b, int S) {
+    if (lengths == nullptr) return S;
+    const int l = lengths[b];
+    return l < 0 ? 0 : (l > S ? S : l);
+}
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// 2^v on the transcendental unit (results below 2^-126 become 0: a decay that small has emptied the state either way)
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * v)); }
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| <= 1, by log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the odd series up to s^15
+// is off by less than s^16 / 17 < 2e-9 of the value for every e, where a logarithm of the rounded 1 + e loses what a small e says
+__device__ __forceinline__ float softplus(float v) {
+    const float e = exp2_fast(-LOG2E * fabsf(v)), s = e * __builtin_amdgcn_rcpf(2.f + e), w = s * s;
+    float q = 1.f / 15.f;
+    q = fmaf(q, w, 1.f / 13.f);
+    q = fmaf(q, w, 1.f / 11.f);
+    q = fmaf(q, w, 1.f / 9.f);
+    q = fmaf(q, w, 1.f / 7.f);
+    q = fmaf(q, w, 1.f / 5.f);
+    q = fmaf(q, w, 1.f / 3.f);
+    q = fmaf(q, w, 1.f);
+    return fmaf(2.f * s, q, fmaxf(v, 0.f));
+}
+
+// ---- sums over a wave's lanes ----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float dpp_mirror(float v) {  // lane ^ 15
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float dpp_half_mirror(float v) {  // lane ^ 7
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float dpp_xor3(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x1b, 0xf, 0xf, true)); }
+__device__ __forceinline__ float dpp_xor1(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true)); }
+
+// Sums of 2 NP values over the 64 lanes, formed as the values appear: f(n, b, c) gives the pair (b_n, c_n).  Each level adds the two halves of a
+// lane group and keeps one of two sums in either half, so the pairs merge as soon as both exist - about 2 instructions a value (a butterfly
+// each would take 6) and a handful of registers.  gfx950's lane swaps exchange the halves of two registers in one instruction; inside a row
+// of 16 lanes the partners are mirrors (DPP).  Lane l returns value l / (32 / NP): b_0.., then c_0.. .
+template <int I> struct Idx { static constexpr int v = I; };
+template <int NP, int LVL, int I, class F>
+__device__ __forceinline__ float pair_tree(F& f, int lane) {
+    if constexpr (LVL == 0) {
+        float b, c;
+        f(Idx<I>{}, b, c);
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(b), __float_as_uint(c), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        const float lo = pair_tree<NP, LVL - 1, I>(f, lane), hi = pair_tree<NP, LVL - 1, I + (NP >> LVL)>(f, lane);
+        if constexpr (LVL == 1) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+            return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        if constexpr (LVL == 2) return ((lane & 8) ? hi : lo) + dpp_mirror((lane & 8) ? lo : hi);
+        if constexpr (LVL == 3) return ((lane & 4) ? hi : lo) + dpp_half_mirror((lane & 4) ? lo : hi);
+        if constexpr (LVL == 4) return ((lane & 2) ? hi : lo) + dpp_xor3((lane & 2) ? lo : hi);
+        if constexpr (LVL == 5) return ((lane & 1) ? hi : lo) + dpp_xor1((lane & 1) ? lo : hi);
+    }
+}
+template <int NP, class F>
+__device__ __forceinline__ float pair_sums(F& f, int lane) {
+    static_assert(NP == 8 || NP == 16 || NP == 32, "8, 16 or 32 pairs");
+    if constexpr (NP == 32) return pair_tree<32, 5, 0>(f, lane);
+    if constexpr (NP == 16) {
+        const float v = pair_tree<16, 4, 0>(f, lane);
+        return v + dpp_xor1(v);
+    }
+    float v = pair_tree<8, 3, 0>(f, lane);
+    v += dpp_xor3(v);
+    return v + dpp_xor1(v);
+}
+
+// The gradients of one network's weights: the partial sums [agent][slot][rows + extra][C] of its agents, in order.  The first `rows` rows go
+// to d0, the next to d1, the one after that to d2 (NULL: not wanted).
+static __global__ __launch_bounds__(256) void ssm_weights_sum_kernel(SsmDims d, int slots, int rows, int extra, const float* __restrict__ part,
+                                                                     float* __restrict__ d0, float* __restrict__ d1, float* __restrict__ d2) {
+    const int m = blockIdx.y;
+    const int64_t n = (int64_t)(rows + extra) * d.C;
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (i < n)
+        for (int p = 0; p < d.P; ++p)
+            if (d.net[p] == m)
+                for (int k = q; k < slots; k += 4) s += part[((int64_t)p * slots + k) * n + i];
+    red[q][lane] = s;
+    __syncthreads();
+    if (q != 0 || i >= n) return;
+    s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    const int64_t r = i / d.C, c = i % d.C;
+    if (r < rows) d0[((int64_t)m * rows + r) * d.C + c] = s;
+    else if (r == rows) { if (d1 != nullptr) d1[(int64_t)m * d.C + c] = s; }
+    else if (d2 != nullptr) d2[(int64_t)m * d.C + c] = s;
+}
+
+// order LDS traffic between the lanes of ONE wave (the queue itself is in order; this holds the compiler to it)
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+}  // namespace marl

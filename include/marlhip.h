@@ -839,6 +839,99 @@ int marlhip_qmix_update_n(const marlhip_qmix_learner* L, int32_t n_updates, int3
                           void* exchange_ctx, int32_t world, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * State space sequence operators: the selective scan and its short causal convolution, the recurrent mixing of a state space agent network
+ * next to the GRU sequences above (marlhip_gru_forward: same [agent][step][row] layout, same carried state between calls).  They have no
+ * counterpart in the reference, whose recurrent networks are GRUs (marlbase/utils/models.py:74-90).
+ *
+ * Sequences: element (p, t, b, c) at data + p * agent_stride + t * step_stride + b * row_stride + c, strides in ELEMENTS, any value
+ * (slices of wider projections, broadcast strides 0 for inputs); data == NULL: absent.  Outputs are contiguous [P][S][B][C].
+ *   dtype: 0 f32, 1 bf16, 2 f16 - of every sequence, its gradient and the convolution's window; weights, their gradients and the scan's
+ *   state are f32, and so is all arithmetic: a result is rounded once, when it is stored.
+ *   weights are per network ([M][..][C]); net_of maps agents to networks as in marlhip_net_shape (n_networks == 0: one network an agent).
+ *   reset u8 [S][B] or NULL: an episode starts at step t of row b - the state is zero before it, the window empty.
+ *   lengths i32 [B] or NULL: steps of row b (clamped to 0..S).  Steps behind the end are not read; their outputs are 0 and the carried
+ *   state is the one after the last step that counts.
+ *   The carried state may be updated in place (h_out == h_in, state_out == state).
+ *
+ * Sums have a fixed order: equal inputs give equal bits.  Any S and B >= 0, C >= 1.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct marlhip_ssm_shape {
+    int32_t n_agents, steps, batch, channels; /* P (1..16), S, B, C */
+    int32_t state;                            /* scan: N states a channel (1..32); convolution: W taps (1..8) */
+    int32_t groups;                           /* scan: G groups of C / G channels share B and C; convolution: 1 */
+    int32_t dtype;
+    int32_t n_networks;
+    int32_t net_of[16];
+} marlhip_ssm_shape;
+
+typedef struct marlhip_ssm_seq {
+    const void* data;
+    int64_t agent_stride, step_stride, row_stride;
+} marlhip_ssm_seq;
+
+/* y_t = silu(bias + sum_k weight[k] x_{t-W+1+k}) (silu == 0: without the activation); the window before step 0 is `state`
+ * [P][B][W-1][C], oldest first (NULL: zeros); state_out (NULL: not wanted) receives the last W-1 inputs, those of an episode that a
+ * reset ended as zeros. */
+typedef struct marlhip_ssm_conv_args {
+    marlhip_ssm_seq x, dy;       /* dy: gradient calls */
+    const float *weight, *bias;  /* [M][W][C], [M][C] or NULL */
+    int32_t silu;
+    const void* state;
+    const uint8_t* reset;
+    const int32_t* lengths;
+    void *y, *state_out;
+    const void* dstate_out;      /* gradient call: [P][B][W-1][C] gradient at state_out, or NULL (zeros) */
+    void *dx, *dstate;           /* contiguous; dstate: NULL if not wanted */
+    float *dweight, *dbias;      /* [M][W][C], [M][C] (dbias: NULL without bias) */
+} marlhip_ssm_conv_args;
+int marlhip_ssm_conv(const marlhip_ssm_shape* s, const marlhip_ssm_conv_args* a, void* stream);
+int64_t marlhip_ssm_conv_grad_workspace_bytes(const marlhip_ssm_shape* s);
+int marlhip_ssm_conv_grad(const marlhip_ssm_shape* s, const marlhip_ssm_conv_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dt = softplus(delta + delta_bias) (softplus == 0: dt = delta + delta_bias); h_t = exp(dt A) h_{t-1} + dt B_t x_t;
+ * y_t = (C_t . h_t + D x_t) silu(z_t) (z absent: no gate).  A [M][N][C] is the decay rate itself (negative for a decaying state).
+ * B, C: [..][G][N] at (p, t, b), the last two dimensions contiguous.  h [P][B][N][C] f32.
+ * record (NULL or marlhip_ssm_scan_record_floats floats): the states the backward pass starts its blocks of steps from, written by the
+ * forward call with the SAME arguments. */
+typedef struct marlhip_ssm_scan_args {
+    marlhip_ssm_seq x, delta, B, C, z, dy;  /* dy: gradient calls */
+    const float *A, *D, *delta_bias;        /* [M][N][C], [M][C] or NULL, [M][C] or NULL */
+    int32_t softplus;
+    const float* h_in;                      /* NULL: zeros */
+    const uint8_t* reset;
+    const int32_t* lengths;
+    void* y;
+    float *h_out, *record;                  /* h_out: NULL if not wanted; record: written by the forward call, read by the gradient */
+    const float* dh_out;                    /* gradient at h_out, or NULL (zeros) */
+    void *dx, *ddelta, *dB, *dC, *dz;       /* contiguous [P][S][B][C], dB / dC [P][S][B][G][N]; dz: NULL without z */
+    float *dA, *dD, *ddelta_bias, *dh_in;   /* dD / ddelta_bias: NULL without D / delta_bias; dh_in: NULL if not wanted */
+} marlhip_ssm_scan_args;
+int64_t marlhip_ssm_scan_record_floats(const marlhip_ssm_shape* s);
+int64_t marlhip_ssm_scan_workspace_bytes(const marlhip_ssm_shape* s);
+int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t marlhip_ssm_scan_grad_workspace_bytes(const marlhip_ssm_shape* s);
+int marlhip_ssm_scan_grad(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Global gradient norm over many tensors and the clip (torch.nn.utils.clip_grad_norm_, which the reference calls on its parameter list:
+ * dqn/model.py:170; marlhip_dqn_clip_adam does it for one flat block).
+ * tensors[i]: n elements at data, contiguous; clip: data * min(max_norm / (norm + 1e-6), 1) goes to out (NULL: in place), rounded once to
+ * the tensor's type.  The squares are summed in 64 bits in a fixed order; norm_out[0] (device) is the norm before the clip.  A norm that is
+ * not finite scales by 0 (infinity) or NaN as there.  The tensors must not overlap each other; `tensors` itself is HOST memory, read
+ * during the call.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct marlhip_tensor {
+    const void* data;
+    void* out;      /* clip: destination, NULL = data */
+    int64_t n;
+    int32_t dtype;  /* 0 f32, 1 bf16, 2 f16 */
+} marlhip_tensor;
+int64_t marlhip_grad_norm_workspace_bytes(const marlhip_tensor* tensors, int32_t count);
+int marlhip_grad_norm(const marlhip_tensor* tensors, int32_t count, float* norm_out, void* workspace, int64_t workspace_bytes, void* stream);
+int marlhip_clip_grad_norm(const marlhip_tensor* tensors, int32_t count, float max_norm, float* norm_out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Measurement aid (bench.py roofline leg): when enabled, the named kernels are bracketed by HIP
  * events on the stream they are launched on.  ids: 0 loss/grad kernel, 1 fused collector,
  * 2 replay sample gather, 3 env step, 4 QMIX mixer stage, 5 the gradient exchange of the data-parallel update loops (the reduce launch

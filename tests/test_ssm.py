@@ -1,0 +1,837 @@
+"""State space sequence operators (hip.ssm_conv / ssm_scan and their gradients) against their definition in 64 bits.
+
+Tolerances.  Every result is a sum of products; `mag` is the sum of the products' magnitudes, taken from the same reference on absolute
+values.  With u = 2^-24 (half an f32 step) an f32 evaluation is off by at most u * mag times the number of roundings on a term's way to the
+result.  A term passes at most S decays, each one product, one exponential of a rounded exponent (relative error |dt A| u, and the decay it
+multiplies with bounds the sum of these over the steps) and one addition: 4 S roundings.  softplus, sigmoid, the dot product over N <= 32 states and the
+cross-lane sums over C <= 64 G channels a block add less than 128.  Weight gradients add up S * B terms one by one at worst.  A result of a
+16-bit type is rounded once more, by half a step of its type."""
+import itertools
+
+import pytest
+import torch
+
+from codebase_amd import hip as h
+
+U = 2.0**-24
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+TINY = {torch.float32: 1e-37, torch.bfloat16: 1e-37, torch.float16: 2.0**-25}  # half a step at the bottom of the range
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def close(got, ref, mag, roundings, what):
+    assert tuple(got.shape) == tuple(ref.shape), (what, got.shape, ref.shape)
+    if got.numel() == 0:
+        return
+    ref, mag = ref.double(), mag.double().abs()
+    bound = U * roundings * mag + HALF[got.dtype] * (ref.abs() + U * roundings * mag) + TINY[got.dtype]
+    err = (got.double() - ref).abs()
+    assert bool(torch.isfinite(got).all()), f"{what}: not finite"
+    worst = (err / bound).max().item()
+    assert worst <= 1.0, f"{what}: error {err.max().item():.3e} is {worst:.2f} times its bound"
+
+
+# ---- the definitions in 64 bits -----------------------------------------------------------------------------------------------------
+def live_and_fresh(S, B, reset, lengths, dev):
+    t = torch.arange(S, device=dev)[:, None]
+    live = torch.ones(S, B, dtype=torch.bool, device=dev) if lengths is None else t < lengths.long().clamp(0, S)[None]
+    fresh = torch.zeros(S, B, dtype=torch.bool, device=dev) if reset is None else (reset != 0)
+    return live, fresh & live
+
+
+def scan_core(x, dtu, dta, A, Bm, Cm, D, h0, live, fresh):
+    """h_t = exp(dta A) h + dtu B x, ys_t = C.h + D x; x.. [P][S][B][C], A [P][N][C], Bm / Cm [P][S][B][N][C]"""
+    hcur, ys = h0, []
+    for t in range(x.shape[1]):
+        lv, fr = live[t][None, :, None, None], fresh[t][None, :, None, None]
+        hp = torch.where(fr, torch.zeros_like(hcur), hcur)
+        hn = torch.exp(dta[:, t, :, None, :] * A[:, None]) * hp + (dtu[:, t] * x[:, t])[:, :, None, :] * Bm[:, t]
+        yt = (Cm[:, t] * hn).sum(2) + D[:, None, :] * x[:, t]
+        ys.append(torch.where(lv[:, :, 0], yt, torch.zeros_like(yt)))
+        hcur = torch.where(lv, hn, hcur)
+    return (torch.stack(ys, 1) if ys else torch.zeros_like(x)), hcur
+
+
+def scan_reference(v, grads=True):
+    """v: dict of the call's arguments -> {name: (value, magnitude)}"""
+    x = v["x"]
+    P, S, B, C = x.shape
+    N, G, dev = v["A"].shape[1], v["B"].shape[3], x.device
+    net = torch.tensor(v["sharing"] if v["sharing"] is not None else range(P), device=dev)
+    M = v["A"].shape[0]
+    live, fresh = live_and_fresh(S, B, v["reset"], v["lengths"], dev)
+    lv = live[None, :, :, None]
+
+    def clean(t):  # steps behind the end are not looked at
+        return torch.where(lv if t.dim() == 4 else lv[..., None], t.double(), torch.zeros((), dtype=torch.float64, device=dev))
+
+    def wide(m):
+        return clean(m).transpose(-1, -2).repeat_interleave(C // G, -1)
+
+    zero = torch.zeros((), dtype=torch.float64, device=dev)
+    A = v["A"].double()[net]
+    D = v["D"].double()[net] if v["D"] is not None else torch.zeros(P, C, dtype=torch.float64, device=dev)
+    raw = clean(v["delta"]) + (v["delta_bias"].double()[net][:, None, None, :] if v["delta_bias"] is not None else 0.0)
+    dt = torch.where(lv, torch.nn.functional.softplus(raw, threshold=100.0) if v["softplus"] else raw, zero)
+    ddt = torch.where(lv, torch.sigmoid(raw) if v["softplus"] else torch.ones_like(raw), zero)
+    gate = dgate = None
+    if v["z"] is not None:
+        z = clean(v["z"])
+        sg = torch.sigmoid(z)
+        gate, dgate = z * sg, sg * (1 + z * (1 - sg))
+    h0 = v["h_in"].double() if v["h_in"] is not None else torch.zeros(P, B, N, C, dtype=torch.float64, device=dev)
+    out = {}
+    for which in (0, 1):  # the values, their magnitudes
+        f = (lambda t: t) if which == 0 else torch.abs
+        leaf = [f(t).clone().requires_grad_(True) for t in (clean(x), dt, wide(v["B"]), wide(v["C"]), D, h0)]
+        lx, ldu, lB, lC, lD, lh = leaf
+        lda, lA = dt.clone().requires_grad_(True), A.clone().requires_grad_(True)
+        ys, hT = scan_core(lx, ldu, lda, lA, lB, lC, lD, lh, live, fresh)
+        g = torch.ones_like(ys) if gate is None else f(gate)
+        res = {"y": torch.where(lv, ys * g, zero).detach(), "h": hT.detach()}
+        if grads:
+            dy = f(clean(v["dy"]))
+            loss = (dy * g * ys).sum()
+            if v["dh_out"] is not None:
+                loss = loss + (f(v["dh_out"].double()) * hT).sum()
+            if loss.requires_grad:
+                gx, gdu, gda, gA, gB, gC, gD, gh = (torch.zeros_like(a) if q is None else q for a, q in zip(
+                    (lx, ldu, lda, lA, lB, lC, lD, lh), torch.autograd.grad(loss, (lx, ldu, lda, lA, lB, lC, lD, lh), allow_unused=True)))
+            else:
+                gx, gdu, gda, gA, gB, gC, gD, gh = (torch.zeros_like(a) for a in (lx, ldu, lda, lA, lB, lC, lD, lh))
+
+            def narrow(m):
+                return m.unflatten(-1, (G, C // G)).sum(-1).transpose(-1, -2)
+
+            def per_net(m):
+                return torch.zeros(M, *m.shape[1:], dtype=torch.float64, device=dev).index_add_(0, net, m)
+
+            gd = (f(gdu) + f(gda)) * ddt
+            res.update(dx=gx, ddelta=gd, dA=per_net(f(gA)), dB=narrow(gB), dC=narrow(gC), dD=per_net(gD), ddelta_bias=per_net(gd.sum((1, 2))), dh=gh)
+            if gate is not None:
+                # the slope sg + sg z (1 - sg) is itself a sum of two products, which cancel where silu has its minimum (z = -1.278): with either
+                # one rounded to a relative u the slope is off by u times the sum of their magnitudes, whatever is left of it
+                slope = dgate if which == 0 else sg * (1 + z.abs() * (1 - sg))
+                res["dz"] = dy * ys.detach() * slope
+        for k, t in res.items():
+            out[k] = (t,) if which == 0 else (out[k][0], t)
+    return out
+
+
+def make_scan(P, S, B, C, N, G=1, dtype=F32, sharing=None, z=True, D=True, bias=True, softplus=True, carry=True, reset=True, lengths=True,
+              seed=0, device="cuda", rate=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    M = P if sharing is None else max(sharing) + 1
+
+    def rn(*s, scale=1.0, dt=dtype):
+        return (torch.randn(*s, generator=gen) * scale).to(dt).to(device)
+
+    v = dict(sharing=sharing, softplus=softplus)
+    xz = rn(P, S, B, 2 * C)
+    maps = rn(P, S, B, 3 + 2 * G * N)
+    v["x"], v["z"] = xz[..., :C], (xz[..., C:] if z else None)
+    v["B"], v["C"] = maps[..., 3:3 + G * N].unflatten(-1, (G, N)), maps[..., 3 + G * N:].unflatten(-1, (G, N))
+    v["delta"] = rn(P, S, B, C, scale=0.5) if softplus else rn(P, S, B, C, scale=0.1).abs()
+    v["A"] = -(0.2 + torch.rand(M, N, C, generator=gen) * 4.0 * rate).to(device)
+    v["D"] = rn(M, C, dt=F32) if D else None
+    v["delta_bias"] = rn(M, C, scale=0.5, dt=F32) - (1.5 if softplus else 0.0) if bias else None
+    if bias and not softplus:
+        v["delta_bias"] = v["delta_bias"].abs() * 0.1
+    v["h_in"] = rn(P, B, N, C, dt=F32) if carry else None
+    v["reset"] = (torch.rand(S, B, generator=gen) < 0.2).to(torch.uint8).to(device) if reset else None
+    v["lengths"] = torch.randint(0, S + 1, (B,), generator=gen).to(torch.int32).to(device) if lengths else None
+    v["dy"] = rn(P, S, B, C)
+    v["dh_out"] = rn(P, B, N, C, dt=F32) if carry else None
+    return v
+
+
+def scan_call(v, record=None, **kw):
+    k = {n: v[n] for n in ("D", "z", "delta_bias", "softplus", "sharing", "h_in", "reset", "lengths")}
+    k.update(kw)
+    return h.ssm_scan(v["x"], v["delta"], v["A"], v["B"], v["C"], record=record, **k)
+
+
+def scan_grad_call(v, record):
+    k = {n: v[n] for n in ("D", "z", "delta_bias", "softplus", "sharing", "h_in", "reset", "lengths")}
+    return h.ssm_scan_grad(v["dy"], v["x"], v["delta"], v["A"], v["B"], v["C"], record, dh_out=v["dh_out"], **k)
+
+
+def check_scan(v, grads=True):
+    S, B = v["x"].shape[1:3]
+    record = h.ssm_scan_record(v["x"], v["A"].shape[1]) if grads else None
+    y, hT = scan_call(v, record=record, want_h=True)
+    ref = scan_reference(v, grads)
+    n = 4 * S + 128
+    close(y, *ref["y"], n, "y")
+    close(hT, *ref["h"], n, "h")
+    if not grads:
+        return y, hT, None
+    g = scan_grad_call(v, record)
+    for name, t in (("dx", g.x), ("ddelta", g.delta), ("dB", g.B), ("dC", g.C), ("dz", g.z), ("dh", g.h_in)):
+        if t is not None:
+            close(t, *ref[name], 2 * n, name)
+    for name, t in (("dA", g.A), ("dD", g.D), ("ddelta_bias", g.delta_bias)):
+        if t is not None:
+            close(t, *ref[name], 2 * n + S * B * v["x"].shape[0], name)
+    for name, a in (("z", g.z), ("D", g.D), ("delta_bias", g.delta_bias), ("h_in", g.h_in)):
+        assert (a is None) == (v[name] is None)
+    return y, hT, g
+
+
+SHAPES = [  # P, S, B, C, N, G
+    (1, 1, 1, 1, 1, 1), (2, 1, 5, 64, 16, 1), (1, 7, 3, 63, 16, 1), (2, 8, 2, 65, 8, 1), (1, 9, 4, 128, 16, 1), (3, 26, 3, 40, 5, 1),
+    (1, 33, 2, 130, 16, 2), (2, 17, 2, 96, 24, 3), (1, 19, 2, 200, 32, 1), (1, 40, 1, 12, 17, 1), (1, 5, 2, 66, 9, 1),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_scan_and_gradients(shape, dtype):
+    check_scan(make_scan(*shape, dtype=dtype, seed=sum(shape)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("z,D,bias,softplus", list(itertools.product([False, True], repeat=4)))
+def test_scan_optional_arguments(z, D, bias, softplus):
+    check_scan(make_scan(2, 11, 3, 70, 6, z=z, D=D, bias=bias, softplus=softplus, carry=z, reset=D, lengths=bias))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sharing", [(0, 0, 0), (0, 1, 0), (1, 0, 2)])
+def test_scan_networks_shared_between_agents(sharing):
+    check_scan(make_scan(3, 12, 4, 72, 16, sharing=sharing))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,B,C,N", [(200, 1, 64, 16), (333, 2, 72, 8), (130, 1, 20, 32)])
+def test_scan_long_sequences(S, B, C, N):
+    check_scan(make_scan(1, S, B, C, N, rate=0.1, reset=False, lengths=False))
+    check_scan(make_scan(1, S, B, C, N, dtype=BF16, seed=1))
+
+
+@pytest.mark.gpu
+def test_scan_many_rows():
+    """more rows than waves: a wave takes several, and its sums over them stay in registers"""
+    check_scan(make_scan(2, 4, 5000, 16, 4, seed=3))
+
+
+@pytest.mark.gpu
+def test_scan_of_nothing():
+    for P, S, B in ((2, 0, 3), (2, 4, 0), (1, 0, 0)):
+        v = make_scan(P, S, B, 20, 4, reset=False, lengths=False)
+        y, hT, g = check_scan(v)
+        if S == 0:
+            assert torch.equal(hT, v["h_in"]) and torch.equal(g.h_in, v["dh_out"])
+        assert not g.A.any() and not g.D.any() and not g.delta_bias.any()
+
+
+@pytest.mark.gpu
+def test_scan_lengths_beyond_the_range_are_clamped():
+    v = make_scan(1, 6, 4, 10, 3, reset=False, lengths=False)
+    v["lengths"] = torch.tensor([-3, 0, 6, 99], dtype=torch.int32, device="cuda")
+    check_scan(v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scan_does_not_look_behind_the_end(dtype):
+    v = make_scan(2, 13, 5, 70, 7, dtype=dtype, reset=False)
+    live, _ = live_and_fresh(13, 5, None, v["lengths"], "cuda")
+    y0, h0, g0 = check_scan(v)
+    for k in ("x", "z", "delta", "B", "C", "dy"):
+        v[k] = v[k].clone()
+        v[k][:, ~live] = float("nan")
+    record = h.ssm_scan_record(v["x"], 7)
+    y1, h1 = scan_call(v, record=record, want_h=True)
+    g1 = scan_grad_call(v, record)
+    assert torch.equal(y0, y1) and torch.equal(h0, h1)
+    for a, b in zip(g0, g1):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_a_reset_stops_what_is_not_finite(bad):
+    """an episode that ended in infinities leaves the next one's outputs and gradients alone, and the other way round"""
+    v = make_scan(1, 21, 2, 66, 16, reset=False, lengths=False)
+    v["reset"] = torch.zeros(21, 2, dtype=torch.uint8, device="cuda")
+    v["reset"][9] = 1
+    late = {k: (t[:, 9:] if k in ("x", "z", "delta", "B", "C", "dy") else (t[9:] if k == "reset" else t)) for k, t in v.items()}
+    rec = h.ssm_scan_record(late["x"], 16)
+    yl, hl = scan_call(late, record=rec, want_h=True)
+    gl = scan_grad_call(late, rec)
+    w = dict(v)
+    w["x"] = v["x"].clone()
+    w["x"][:, 4] = bad
+    rec = h.ssm_scan_record(w["x"], 16)
+    y, hT = scan_call(w, record=rec, want_h=True)
+    g = scan_grad_call(w, rec)
+    # where blocks of steps start does not change a step's arithmetic: same bits
+    assert torch.equal(y[:, 9:], yl) and torch.equal(hT, hl)
+    assert torch.equal(g.x[:, 9:], gl.x) and torch.equal(g.B[:, 9:], gl.B) and torch.equal(g.delta[:, 9:], gl.delta)
+    w = dict(v)
+    w["dy"] = v["dy"].clone()
+    w["dy"][:, 12] = bad
+    rec = h.ssm_scan_record(w["x"], 16)
+    scan_call(w, record=rec)
+    g1 = scan_grad_call(w, rec)
+    rec = h.ssm_scan_record(v["x"], 16)
+    scan_call(v, record=rec)
+    g0 = scan_grad_call(v, rec)
+    assert torch.equal(g1.x[:, :9], g0.x[:, :9]) and torch.equal(g1.h_in, g0.h_in) and torch.equal(g1.delta[:, :9], g0.delta[:, :9])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_step_by_step_in_place(dtype):
+    """acting: one step a call with the state updated in place"""
+    v = make_scan(2, 14, 6, 80, 16, dtype=dtype, lengths=False)
+    ref = scan_reference(v, grads=False)
+    state = v["h_in"].clone()
+    for t in range(14):
+        w = {k: (a[:, t:t + 1] if k in ("x", "z", "delta", "B", "C") else (a[t:t + 1] if k == "reset" else a)) for k, a in v.items()}
+        yt = scan_call(w, h_in=state, h_out=state)
+        close(yt, *(r[:, t:t + 1] for r in ref["y"]), 4 * 14 + 128, f"step {t}")
+    close(state, *ref["h"], 4 * 14 + 128, "state")
+
+
+@pytest.mark.gpu
+def test_scan_expanded_inputs_and_odd_strides():
+    v = make_scan(2, 9, 6, 68, 6, dtype=BF16, lengths=False)
+    v["B"] = v["B"][:, :, :1].expand(-1, -1, 6, -1, -1)
+    v["C"] = v["C"][:, :1].expand(-1, 9, -1, -1, -1)
+    v["z"] = v["z"][:1].expand(2, -1, -1, -1)
+    v["x"] = torch.randn(9, 2, 6, 71, device="cuda").to(BF16).permute(1, 0, 2, 3)[..., 1:69]
+    v["dy"] = v["dy"].flip(1).transpose(1, 2).contiguous().transpose(1, 2)
+    check_scan(v)
+
+
+@pytest.mark.gpu
+def test_scan_offsets_beyond_32_bits():
+    """steps 2^30 elements apart: the last one starts 6 GiB into the buffer"""
+    P, S, B, C, N = 1, 4, 2, 66, 5
+    v = make_scan(P, S, B, C, N, dtype=BF16)
+    big = torch.empty(3 * 2**30 + B * C, dtype=BF16, device="cuda")
+    x = big.as_strided((P, S, B, C), (0, 2**30, C, 1))
+    x.copy_(v["x"])
+    v["x"] = x
+    check_scan(v)
+
+
+@pytest.mark.gpu
+def test_scan_same_bits_every_time():
+    v = make_scan(2, 40, 37, 100, 16, dtype=BF16)
+    runs = []
+    for _ in range(3):
+        rec = h.ssm_scan_record(v["x"], 16)
+        y, hT = scan_call(v, record=rec, want_h=True)
+        runs.append((y, hT, *[t for t in scan_grad_call(v, rec)]))
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], r))
+
+
+@pytest.mark.gpu
+def test_scan_gradient_against_differences():
+    """the directional derivative of the 64-bit loss along the gradient's own direction"""
+    v = make_scan(1, 10, 3, 20, 4, lengths=False)
+    rec = h.ssm_scan_record(v["x"], 4)
+    scan_call(v, record=rec)
+    g = scan_grad_call(v, rec)
+    lead = dict(x=g.x, delta=g.delta, A=g.A, B=g.B, C=g.C, D=g.D, z=g.z, delta_bias=g.delta_bias, h_in=g.h_in)
+
+    def loss(w):
+        ref = scan_reference(w, grads=False)
+        return ((ref["y"][0] * v["dy"].double()).sum() + (ref["h"][0] * v["dh_out"].double()).sum()).item()
+
+    for name, grad in lead.items():
+        d = grad.double()
+        step = 1e-4 / max(d.abs().max().item(), 1.0)
+        plus, minus = dict(v), dict(v)
+        plus[name], minus[name] = v[name].double() + step * d, v[name].double() - step * d
+        slope, want = (loss(plus) - loss(minus)) / (2 * step), (d * d).sum().item()
+        # third derivatives times step^2 / 6 stay below 1e-6 of the slope; the gradient itself is off by 2 (4 S + 128) u of its terms
+        assert abs(slope - want) <= 1e-4 * abs(want), (name, slope, want)
+
+
+# ---- the convolution ------------------------------------------------------------------------------------------------------------------
+def conv_reference(v, grads=True):
+    x = v["x"]
+    P, S, B, C = x.shape
+    W, dev = v["weight"].shape[1], x.device
+    net = torch.tensor(v["sharing"] if v["sharing"] is not None else range(P), device=dev)
+    M = v["weight"].shape[0]
+    live, fresh = live_and_fresh(S, B, v["reset"], v["lengths"], dev)
+    zero = torch.zeros((), dtype=torch.float64, device=dev)
+    out = {}
+    for which in (0, 1):
+        f = (lambda t: t) if which == 0 else torch.abs
+        lx = f(torch.where(live[None, :, :, None], x.double(), zero)).clone().requires_grad_(True)
+        lw = f(v["weight"].double()[net]).clone().requires_grad_(True)
+        lb = f(v["bias"].double()[net] if v["bias"] is not None else torch.zeros(P, C, dtype=torch.float64, device=dev)).clone().requires_grad_(True)
+        ls = f(v["state"].double() if v["state"] is not None else torch.zeros(P, B, W - 1, C, dtype=torch.float64, device=dev)).clone().requires_grad_(True)
+        win, pres, wins = [ls[:, :, i] for i in range(W - 1)], [], []
+        for t in range(S):
+            lv, fr = live[t][None, :, None], fresh[t][None, :, None]
+            taps = [torch.where(fr, torch.zeros_like(q), q) for q in win] + [lx[:, t]]
+            pres.append(lb[:, None, :] + sum(q * lw[:, i][:, None, :] for i, q in enumerate(taps)))
+            win = [torch.where(lv, n, q) for n, q in zip(taps[1:], win)]
+        pre = torch.stack(pres, 1) if pres else torch.zeros(P, S, B, C, dtype=torch.float64, device=dev)
+        if which == 0:
+            true_pre = pre.detach()
+        sg = torch.sigmoid(true_pre)
+        act = true_pre * sg if v["silu"] else true_pre
+        lvv = live[None, :, :, None]
+        state = torch.stack(win, 2) if W > 1 else ls
+        # |d silu| <= 1.1, so an error of the sum reaches the result at most that much larger; |silu(s)| <= |s|
+        res = {"y": torch.where(lvv, act if which == 0 else 1.1 * pre, zero).detach(), "state": state.detach()}
+        if grads:
+            dact = sg * (1 + true_pre * (1 - sg)) if v["silu"] else torch.ones_like(sg)
+            dy = torch.where(lvv, v["dy"].double(), zero)
+            # |d2 silu| <= 1/2: an error of the sum, at most that of its magnitude, in the slope
+            dpre = dy * dact if which == 0 else dy.abs() * (1.1 + 0.5 * pre.detach())
+            loss = (dpre * pre).sum()
+            if v["dstate_out"] is not None and W > 1:
+                loss = loss + (f(v["dstate_out"].double()) * state).sum()
+            gs = torch.autograd.grad(loss, (lx, lw, lb, ls), allow_unused=True) if loss.requires_grad else (None,) * 4
+            gx, gw, gb, gst = (torch.zeros_like(a) if q is None else q for a, q in zip((lx, lw, lb, ls), gs))
+
+            def per_net(m):
+                return torch.zeros(M, *m.shape[1:], dtype=torch.float64, device=dev).index_add_(0, net, m)
+
+            res.update(dx=gx, dweight=per_net(gw), dbias=per_net(gb), dstate=gst)
+        for k, t in res.items():
+            out[k] = (t,) if which == 0 else (out[k][0], t)
+    return out
+
+
+def make_conv(P, S, B, C, W, dtype=F32, sharing=None, bias=True, silu=True, carry=True, reset=True, lengths=True, seed=0, device="cuda", pad=0):
+    gen = torch.Generator().manual_seed(seed)
+    M = P if sharing is None else max(sharing) + 1
+
+    def rn(*s, scale=1.0, dt=dtype):
+        return (torch.randn(*s, generator=gen) * scale).to(dt).to(device)
+
+    v = dict(sharing=sharing, silu=silu)
+    v["x"] = rn(P, S, B, 2 * C + pad)[..., pad:pad + C]
+    v["weight"], v["bias"] = rn(M, W, C, scale=0.5, dt=F32), (rn(M, C, dt=F32) if bias else None)
+    v["state"] = rn(P, B, W - 1, C) if carry else None
+    v["reset"] = (torch.rand(S, B, generator=gen) < 0.2).to(torch.uint8).to(device) if reset else None
+    v["lengths"] = torch.randint(0, S + 1, (B,), generator=gen).to(torch.int32).to(device) if lengths else None
+    v["dy"], v["dstate_out"] = rn(P, S, B, C), (rn(P, B, W - 1, C) if carry else None)
+    return v
+
+
+def conv_call(v, **kw):
+    k = {n: v[n] for n in ("bias", "silu", "sharing", "state", "reset", "lengths")}
+    k.update(kw)
+    return h.ssm_conv(v["x"], v["weight"], **k)
+
+
+def conv_grad_call(v):
+    k = {n: v[n] for n in ("bias", "silu", "sharing", "state", "reset", "lengths", "dstate_out")}
+    return h.ssm_conv_grad(v["dy"], v["x"], v["weight"], **k)
+
+
+def check_conv(v, grads=True):
+    S, B = v["x"].shape[1:3]
+    y, state = conv_call(v, want_state=True)
+    ref = conv_reference(v, grads)
+    n = 32  # W <= 8 products, the bias, a sigmoid whose exponent is rounded relative to the sum
+    close(y, *ref["y"], n, "y")
+    assert torch.equal(state.double(), ref["state"][0]), "state"  # moved, not computed
+    if not grads:
+        return y, state, None
+    g = conv_grad_call(v)
+    close(g.x, *ref["dx"], 2 * n, "dx")
+    close(g.weight, *ref["dweight"], 2 * n + S * B * v["x"].shape[0], "dweight")
+    if g.bias is not None:
+        close(g.bias, *ref["dbias"], 2 * n + S * B * v["x"].shape[0], "dbias")
+    if g.state is not None:
+        close(g.state, *ref["dstate"], 2 * n, "dstate")
+    assert (g.bias is None) == (v["bias"] is None) and (g.state is None) == (v["state"] is None)
+    return y, state, g
+
+
+CONV_SHAPES = [  # P, S, B, C, W
+    (1, 1, 1, 1, 4), (2, 1, 7, 64, 4), (1, 2, 3, 64, 4), (1, 3, 2, 8, 4), (2, 16, 3, 128, 4), (1, 17, 2, 40, 2), (1, 33, 2, 65, 3), (3, 26, 5, 24, 1), (1, 50, 3, 72, 8),
+    (1, 5, 2, 12, 7), (2, 31, 1, 520, 5), (1, 100, 1, 16, 4),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", CONV_SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_conv_and_gradients(shape, dtype):
+    check_conv(make_conv(*shape, dtype=dtype, seed=sum(shape)))
+    check_conv(make_conv(*shape, dtype=dtype, seed=sum(shape), pad=1))  # not aligned
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias,silu,carry,reset,lengths", list(itertools.product([False, True], repeat=5)))
+def test_conv_optional_arguments(bias, silu, carry, reset, lengths):
+    check_conv(make_conv(2, 19, 3, 24, 4, bias=bias, silu=silu, carry=carry, reset=reset, lengths=lengths))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sharing", [(0, 0, 0), (0, 1, 0), (1, 0, 2)])
+def test_conv_networks_shared_between_agents(sharing):
+    check_conv(make_conv(3, 12, 4, 72, 4, sharing=sharing))
+
+
+@pytest.mark.gpu
+def test_conv_of_nothing():
+    for P, S, B in ((2, 0, 3), (2, 4, 0), (1, 0, 0)):
+        v = make_conv(P, S, B, 20, 4, reset=False, lengths=False)
+        y, state, g = check_conv(v)
+        if S == 0:
+            assert torch.equal(state, v["state"]) and torch.equal(g.state, v["dstate_out"])
+        assert not g.weight.any() and not g.bias.any()
+
+
+@pytest.mark.gpu
+def test_conv_many_rows():
+    check_conv(make_conv(2, 4, 9000, 16, 4, seed=3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_conv_does_not_look_behind_the_end_or_a_reset(bad):
+    v = make_conv(2, 23, 5, 24, 4, reset=False)
+    live, _ = live_and_fresh(23, 5, None, v["lengths"], "cuda")
+    y0, s0, g0 = check_conv(v)
+    w = dict(v)
+    for k in ("x", "dy"):
+        w[k] = v[k].clone()
+        w[k][:, ~live] = bad
+    y1, s1 = conv_call(w, want_state=True)
+    g1 = conv_grad_call(w)
+    assert torch.equal(y0, y1) and torch.equal(s0, s1) and all(torch.equal(a, b) for a, b in zip(g0, g1))
+    v = make_conv(1, 23, 5, 24, 4, reset=False, lengths=False)
+    v["reset"] = torch.zeros(23, 5, dtype=torch.uint8, device="cuda")
+    v["reset"][9] = 1
+    y0, s0, g0 = check_conv(v)
+    w = dict(v)
+    w["x"] = v["x"].clone()
+    w["x"][:, :9] = bad
+    y1 = conv_call(w)
+    g1 = conv_grad_call(w)
+    assert torch.equal(y0[:, 9:], y1[:, 9:]) and torch.equal(g0.x[:, 9:], g1.x[:, 9:])
+    w = dict(v)
+    w["dy"] = v["dy"].clone()
+    w["dy"][:, 9:] = bad
+    assert torch.equal(g0.x[:, :9], conv_grad_call(w).x[:, :9]) and torch.equal(g0.state, conv_grad_call(w).state)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_conv_step_by_step_in_place(dtype):
+    v = make_conv(2, 14, 6, 80, 4, dtype=dtype, lengths=False)
+    y, end = conv_call(v, want_state=True)
+    state = v["state"].clone()
+    for t in range(14):
+        w = dict(v, x=v["x"][:, t:t + 1], reset=v["reset"][t:t + 1])
+        assert torch.equal(conv_call(w, state=state, state_out=state), y[:, t:t + 1])
+    assert torch.equal(state, end)
+
+
+@pytest.mark.gpu
+def test_conv_long_in_place():
+    """a sequence that is worked on in stretches: the window it starts with is read before it is overwritten"""
+    v = make_conv(1, 333, 2, 64, 4, lengths=False)
+    y, end = conv_call(v, want_state=True)
+    state = v["state"].clone()
+    assert torch.equal(conv_call(v, state=state, state_out=state), y) and torch.equal(state, end)
+
+
+@pytest.mark.gpu
+def test_scan_long_in_place():
+    v = make_scan(1, 700, 1, 64, 8, lengths=False)
+    y, end = scan_call(v, want_h=True)
+    state = v["h_in"].clone()
+    assert torch.equal(scan_call(v, h_in=state, h_out=state), y) and torch.equal(state, end)
+
+
+# ---- a recurrent block of them, as it is used ----------------------------------------------------------------------------------------
+def block_weights(P, D, C, N, R, W, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+
+    def rn(*s, scale):
+        return (torch.randn(*s, generator=gen) * scale).cuda()
+
+    return dict(w_in=rn(P, D, 2 * C, scale=D**-0.5), conv=rn(P, W, C, scale=0.5), conv_b=rn(P, C, scale=0.1), w_maps=rn(P, C, R + 2 * N, scale=C**-0.5),
+                w_dt=rn(P, R, C, scale=R**-0.5), dt_b=rn(P, C, scale=0.3) - 2.0, A=-(0.5 + torch.rand(P, N, C, generator=gen) * 4).cuda(),
+                D=rn(P, C, scale=1.0), w_out=rn(P, C, D, scale=C**-0.5))
+
+
+def project(x, w):
+    """[P][S][B][..] times the agent's matrix"""
+    P, S, B, K = x.shape
+    return torch.bmm(x.reshape(P, S * B, K), w.contiguous()).view(P, S, B, -1)
+
+
+@pytest.mark.gpu
+def test_block_trains_and_acts():
+    """projection, convolution, maps, scan, projection: gradients of every weight against 64-bit automatic differentiation of the same block,
+    the clip over all of them, and the sequence against single acting steps"""
+    P, S, B, D, C, N, R, W = 2, 25, 6, 15, 64, 16, 4, 4
+    wt = block_weights(P, D, C, N, R, W)
+    gen = torch.Generator().manual_seed(5)
+    obs, dout = torch.randn(P, S, B, D, generator=gen).cuda(), torch.randn(P, S, B, D, generator=gen).cuda()
+    reset = (torch.rand(S, B, generator=gen) < 0.1).to(torch.uint8).cuda()
+
+    def forward(obs, reset, conv_state=None, h_state=None, record=None):
+        xz = project(obs, wt["w_in"])
+        kw = dict(reset=reset)
+        u = h.ssm_conv(xz[..., :C], wt["conv"], wt["conv_b"], state=conv_state, state_out=conv_state, **kw)
+        maps = project(u, wt["w_maps"])
+        delta = project(maps[..., :R], wt["w_dt"])
+        Bm, Cm = maps[..., R:R + N].unflatten(-1, (1, N)), maps[..., R + N:].unflatten(-1, (1, N))
+        y = h.ssm_scan(u, delta, wt["A"], Bm, Cm, D=wt["D"], z=xz[..., C:], delta_bias=wt["dt_b"], h_in=h_state, h_out=h_state, record=record, **kw)
+        return project(y, wt["w_out"]), (xz, u, maps, delta, Bm, Cm, y)
+
+    record = h.ssm_scan_record(torch.empty(P, S, B, C, device="cuda"), N)
+    out, (xz, u, maps, delta, Bm, Cm, y) = forward(obs, reset, record=record)
+
+    def flat(t):
+        return t.reshape(P, S * B, -1)
+
+    def outer(a, b):  # sum over rows of a^T b
+        return torch.bmm(flat(a).transpose(1, 2).contiguous(), flat(b).contiguous())
+
+    def back(g, w):
+        return project(g, w.transpose(1, 2))
+
+    grads = {"w_out": outer(y, dout)}
+    gs = h.ssm_scan_grad(back(dout, wt["w_out"]), u, delta, wt["A"], Bm, Cm, record, D=wt["D"], z=xz[..., C:], delta_bias=wt["dt_b"], reset=reset)
+    grads.update(A=gs.A, D=gs.D, dt_b=gs.delta_bias, w_dt=outer(maps[..., :R], gs.delta))
+    dmaps = torch.cat([back(gs.delta, wt["w_dt"]), gs.B.flatten(-2), gs.C.flatten(-2)], -1)
+    grads["w_maps"] = outer(u, dmaps)
+    gc = h.ssm_conv_grad(gs.x + back(dmaps, wt["w_maps"]), xz[..., :C], wt["conv"], wt["conv_b"], reset=reset)
+    grads.update(conv=gc.weight, conv_b=gc.bias, w_in=outer(obs, torch.cat([gc.x, gs.z], -1)))
+
+    # the same block in 64 bits, by automatic differentiation
+    ref = {k: t.double().requires_grad_(True) for k, t in wt.items()}
+    fresh = reset != 0
+    xzr = torch.einsum("psbd,pdc->psbc", obs.double(), ref["w_in"])
+    win, us = [torch.zeros(P, B, C, dtype=torch.float64, device="cuda")] * (W - 1), []
+    for t in range(S):
+        win = [torch.where(fresh[t][None, :, None], torch.zeros_like(q), q) for q in win] + [xzr[:, t, :, :C]]
+        s = ref["conv_b"][:, None] + sum(q * ref["conv"][:, i][:, None] for i, q in enumerate(win))
+        us.append(s * torch.sigmoid(s))
+        win = win[1:]
+    ur = torch.stack(us, 1)
+    mr = torch.einsum("psbc,pcr->psbr", ur, ref["w_maps"])
+    dt = torch.nn.functional.softplus(torch.einsum("psbr,prc->psbc", mr[..., :R], ref["w_dt"]) + ref["dt_b"][:, None, None])
+    ys, _ = scan_core(ur, dt, dt, ref["A"], mr[..., R:R + N, None].expand(-1, -1, -1, -1, C), mr[..., R + N:, None].expand(-1, -1, -1, -1, C), ref["D"],
+                      torch.zeros(P, B, N, C, dtype=torch.float64, device="cuda"), torch.ones_like(fresh), fresh)
+    zr = xzr[..., C:]
+    outr = torch.einsum("psbc,pcd->psbd", ys * zr * torch.sigmoid(zr), ref["w_out"])
+    want = dict(zip(ref, torch.autograd.grad((outr * dout.double()).sum(), list(ref.values()))))
+    # f32 through four products of up to S B = 150 terms and the scan: (4 S + 128 + 4 * 150) roundings, of values whose terms cancel to about
+    # 1 / sqrt(150) of their magnitudes' sum
+    tol = U * (4 * S + 128 + 600) * 150**0.5
+    assert (out.double() - outr).abs().max() <= tol * outr.abs().max()
+    for k in want:
+        err = (grads[k].double() - want[k]).abs().max().item() / want[k].abs().max().item()
+        assert err <= tol, (k, err, tol)
+
+    # the clip over all of them
+    total = torch.sqrt(sum((g.double()**2).sum() for g in grads.values()))
+    before = [g.clone() for g in grads.values()]
+    norm = h.clip_grad_norm(list(grads.values()), 1.0)
+    assert abs(norm.item() - total.item()) <= 4 * U * total.item()
+    for b, g in zip(before, grads.values()):
+        close(g, b.double() * (1.0 / (total + 1e-6)), b.double() / total, 8, "clipped")
+
+    # acting, one step a call
+    conv_state, h_state = torch.zeros(P, B, W - 1, C, device="cuda"), torch.zeros(P, B, N, C, device="cuda")
+    for t in range(S):
+        step, _ = forward(obs[:, t:t + 1], reset[t:t + 1], conv_state, h_state)
+        assert (step.double() - outr[:, t:t + 1]).abs().max() <= tol * outr.abs().max()
+
+
+@pytest.mark.gpu
+def test_forward_and_backward_in_a_graph():
+    """captured once, replayed with other inputs and eager calls between the replays: every replay gives the eager bits"""
+    v, c = make_scan(2, 30, 9, 72, 16, seed=1), make_conv(2, 30, 9, 72, 4, seed=2)
+    v["x"], c["x"] = v["x"].contiguous(), c["x"].contiguous()
+
+    def everything():
+        rec = h.ssm_scan_record(v["x"], 16)
+        y, hT = scan_call(v, record=rec, want_h=True)
+        g = scan_grad_call(v, rec)
+        yc, st = conv_call(c, want_state=True)
+        gc = conv_grad_call(c)
+        return [y, hT, *g, yc, st, *gc]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        everything()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = everything()
+    for i in range(4):
+        gen = torch.Generator().manual_seed(100 + i)
+        v["x"].copy_(torch.randn(v["x"].shape, generator=gen))
+        c["x"].copy_(torch.randn(c["x"].shape, generator=gen))
+        want = everything()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), f"replay {i}"
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    a, b = make_scan(2, 60, 40, 72, 16, seed=1), make_scan(1, 50, 64, 100, 8, seed=2)
+
+    def run(v):
+        rec = h.ssm_scan_record(v["x"], v["A"].shape[1])
+        y = scan_call(v, record=rec)
+        return [y, *scan_grad_call(v, rec)]
+
+    want = [run(a), run(b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(3):
+        for k, v in enumerate((a, b)):
+            with torch.cuda.stream(streams[k]):
+                got[k] = run(v)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(g, w) if p is not None)
+
+
+# ---- refusals (no device is touched) -------------------------------------------------------------------------------------------------
+SCAN_BAD = [
+    ("x", lambda v: v["x"][0], "x is not"),
+    ("x", lambda v: v["x"].double(), "not supported"),
+    ("x", lambda v: v["x"].transpose(2, 3).contiguous().transpose(2, 3), "x has stride"),
+    ("delta", lambda v: v["delta"][:, :-1], "delta has shape"),
+    ("delta", lambda v: v["delta"].to(BF16), "delta is torch.bfloat16"),
+    ("B", lambda v: v["B"][:, :, :, 0], "B is not"),
+    ("B", lambda v: v["B"].transpose(3, 4).contiguous().transpose(3, 4), "B has stride"),
+    ("C", lambda v: v["C"][..., :-1], "C has shape"),
+    ("A", lambda v: v["A"][:1], "A has shape"),
+    ("A", lambda v: v["A"].to(BF16), "A is torch.bfloat16"),
+    ("D", lambda v: v["D"][:, :-1], "D has shape"),
+    ("delta_bias", lambda v: v["delta_bias"].double(), "delta_bias is"),
+    ("h_in", lambda v: v["h_in"].to(BF16), "h_in is"),
+    ("h_in", lambda v: v["h_in"].transpose(2, 3).contiguous().transpose(2, 3), "h_in is not contiguous"),
+    ("z", lambda v: v["z"][:, :, :, :-1], "z has shape"),
+    ("reset", lambda v: v["reset"].float(), "reset is"),
+    ("reset", lambda v: v["reset"].t().contiguous(), "reset has shape"),
+    ("lengths", lambda v: v["lengths"].long(), "lengths is"),
+    ("sharing", lambda v: (0, 1, 0), "one per agent"),
+]
+
+
+@pytest.mark.parametrize("name,spoil,text", SCAN_BAD)
+def test_scan_refuses(name, spoil, text):
+    v = make_scan(2, 5, 3, 12, 4, G=2, device="cpu")
+    rec = h.ssm_scan_record(v["x"], 4)
+    v[name] = spoil(v)
+    with pytest.raises(ValueError, match=text):
+        scan_call(v, want_h=True)
+    with pytest.raises(ValueError, match=text):
+        scan_grad_call(v, rec)
+
+
+def test_scan_refuses_sizes_and_states():
+    v = make_scan(2, 5, 3, 12, 4, G=2, device="cpu")
+    with pytest.raises(ValueError, match="record is missing"):
+        scan_grad_call(v, None)
+    with pytest.raises(ValueError, match="record has shape"):
+        scan_grad_call(v, torch.empty(7))
+    with pytest.raises(ValueError, match="h_out has shape"):
+        scan_call(v, h_out=v["h_in"][:1])
+    wide = torch.empty(v["h_in"].numel() + 4)
+    with pytest.raises(ValueError, match="overlaps"):
+        scan_call(v, h_in=wide[:-4].view(v["h_in"].shape), h_out=wide[4:].view(v["h_in"].shape))
+    with pytest.raises(ValueError, match="dy has shape"):
+        scan_grad_call(dict(v, dy=v["dy"][:, 1:]), h.ssm_scan_record(v["x"], 4))
+    with pytest.raises(ValueError, match="dh_out has shape"):
+        scan_grad_call(dict(v, dh_out=v["dh_out"][..., 1:]), h.ssm_scan_record(v["x"], 4))
+    with pytest.raises(h.MarlHipError, match="33 states"):
+        h.ssm_scan_record(v["x"], 33)
+    with pytest.raises(h.MarlHipError, match="17 agents"):
+        h.ssm_scan_record(torch.empty(17, 1, 1, 4), 4)
+    with pytest.raises(h.MarlHipError, match="CPU"):
+        scan_call(v)
+    with pytest.raises(h.MarlHipError, match="CPU"):
+        scan_grad_call(v, h.ssm_scan_record(v["x"], 4))
+
+
+def test_c_entry_points_refuse_bad_shapes():
+    import ctypes
+
+    from codebase_amd import _lib
+
+    lib = _lib.lib
+
+    def shape(**kw):
+        s = _lib.SsmShape(2, 5, 3, 12, 4, 2, 0, 0)
+        for k, val in kw.items():
+            setattr(s, k, val)
+        return s
+
+    for kw, text in ((dict(n_agents=0), "agents"), (dict(steps=-1), "steps"), (dict(batch=-1), "batch"), (dict(channels=0), "channels"), (dict(dtype=3), "dtype"),
+                     (dict(state=0), "states"), (dict(groups=5), "groups"), (dict(n_networks=3), "networks")):
+        s = shape(**kw)
+        for fn in (lib.marlhip_ssm_scan_record_floats, lib.marlhip_ssm_scan_workspace_bytes, lib.marlhip_ssm_scan_grad_workspace_bytes):
+            assert fn(ctypes.byref(s)) < 0 and text in _lib.last_error(), (kw, _lib.last_error())
+        assert lib.marlhip_ssm_scan(ctypes.byref(s), ctypes.byref(_lib.SsmScanArgs()), None, 0, None) < 0
+    for kw, text in ((dict(state=9), "taps"), (dict(state=0), "taps"), (dict(groups=2), "groups")):
+        s = shape(**dict(dict(groups=1), **kw))
+        assert lib.marlhip_ssm_conv_grad_workspace_bytes(ctypes.byref(s)) < 0 and text in _lib.last_error()
+        assert lib.marlhip_ssm_conv(ctypes.byref(s), ctypes.byref(_lib.SsmConvArgs()), None) < 0
+    s = shape()
+    assert lib.marlhip_ssm_scan(ctypes.byref(s), None, None, 0, None) < 0 and "NULL" in _lib.last_error()
+    assert lib.marlhip_ssm_scan(ctypes.byref(s), ctypes.byref(_lib.SsmScanArgs()), None, 0, None) < 0 and "NULL" in _lib.last_error()
+    assert lib.marlhip_ssm_scan(None, ctypes.byref(_lib.SsmScanArgs()), None, 0, None) < 0 and "NULL" in _lib.last_error()
+    bad = shape(n_networks=1)
+    bad.net_of[1] = 1
+    assert lib.marlhip_ssm_scan_record_floats(ctypes.byref(bad)) < 0 and "net_of" in _lib.last_error()
+
+
+CONV_BAD = [
+    ("x", lambda v: v["x"][0], "x is not"),
+    ("x", lambda v: v["x"].to(torch.int32), "not supported"),
+    ("x", lambda v: v["x"].transpose(2, 3).contiguous().transpose(2, 3), "x has stride"),
+    ("weight", lambda v: v["weight"][0], "weight is not"),
+    ("weight", lambda v: v["weight"][..., 1:], "weight has shape"),
+    ("weight", lambda v: v["weight"].to(BF16), "weight is torch.bfloat16"),
+    ("bias", lambda v: v["bias"][:1], "bias has shape"),
+    ("state", lambda v: v["state"][:, :, 1:], "state has shape"),
+    ("state", lambda v: v["state"].to(F16), "state is"),
+    ("reset", lambda v: v["reset"][1:], "reset has shape"),
+    ("lengths", lambda v: v["lengths"].float(), "lengths is"),
+    ("sharing", lambda v: (0,), "one per agent"),
+]
+
+
+@pytest.mark.parametrize("name,spoil,text", CONV_BAD)
+def test_conv_refuses(name, spoil, text):
+    v = make_conv(2, 5, 3, 12, 4, device="cpu")
+    v[name] = spoil(v)
+    with pytest.raises(ValueError, match=text):
+        conv_call(v, want_state=True)
+    with pytest.raises(ValueError, match=text):
+        conv_grad_call(v)
+
+
+def test_conv_refuses_states_and_the_cpu():
+    v = make_conv(2, 5, 3, 12, 4, device="cpu")
+    with pytest.raises(ValueError, match="state_out has shape"):
+        conv_call(v, state_out=v["state"][:1])
+    with pytest.raises(ValueError, match="dstate_out has shape"):
+        conv_grad_call(dict(v, dstate_out=v["state"][:1]))
+    with pytest.raises(h.MarlHipError, match="CPU"):
+        conv_call(v)
+    with pytest.raises(h.MarlHipError, match="9 taps"):
+        big = make_conv(2, 5, 3, 12, 9, device="cpu")
+        h.check(h.lib.marlhip_ssm_conv_grad_workspace_bytes(h._ssm_shape("conv", big["x"], 9, 1, None)[0]))
