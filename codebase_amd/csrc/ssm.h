@@ -29,6 +29,9 @@ __device__ __forceinline__ const T* seq_at(const SsmSeq& s, int p, int b) {
     return static_cast<const T*>(s.data) + p * s.sp + b * s.sb;
 }
 
+constexpr int ROW_MAX = 0x7fffffff;    // bytes of a row descriptor that does not bound its row
+constexpr int OOB = (int)0x80000000;   // an offset behind any row
+
 // One row of a wave through a buffer descriptor: the base is uniform, `bytes` of it exist.  Lanes behind them load 0 and store nothing, and
 // with bytes = 0 a whole row is skipped - no predicate registers, no per-lane 64-bit addresses.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* base, int bytes) {
@@ -113,41 +116,40 @@ __device__ __forceinline__ float dpp_half_mirror(float v) {  // lane ^ 7
 __device__ __forceinline__ float dpp_xor3(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x1b, 0xf, 0xf, true)); }
 __device__ __forceinline__ float dpp_xor1(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true)); }
 
-// Sums of 2 NP values over the 64 lanes, formed as the values appear: f(n, b, c) gives the pair (b_n, c_n).  Each level adds the two halves of a
-// lane group and keeps one of two sums in either half, so the pairs merge as soon as both exist - about 2 instructions a value (a butterfly
-// each would take 6) and a handful of registers.  gfx950's lane swaps exchange the halves of two registers in one instruction; inside a row
-// of 16 lanes the partners are mirrors (DPP).  Lane l returns value l / (32 / NP): b_0.., then c_0.. .
 template <int I> struct Idx { static constexpr int v = I; };
-template <int NP, int LVL, int I, class F>
+
+// keeps one of two sums in either half of a lane group: lanes with `bit` clear return lo, the others hi, each with its partner's share
+template <int BIT>
+__device__ __forceinline__ float half_sum(float lo, float hi, int lane) {
+    if constexpr (BIT == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else if constexpr (BIT == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        const float keep = (lane & BIT) ? hi : lo, give = (lane & BIT) ? lo : hi;
+        if constexpr (BIT == 8) return keep + dpp_mirror(give);
+        if constexpr (BIT == 4) return keep + dpp_half_mirror(give);
+        if constexpr (BIT == 2) return keep + dpp_xor3(give);
+        return keep + dpp_xor1(give);
+    }
+}
+
+// Sums of 8 pairs over the TOP * 2 lanes of a group, formed as the pairs appear: f(n, b, c) gives (b_n, c_n).  The pairs merge as soon as two
+// exist - about 2 instructions a value, where a butterfly each would take 2 log2(lanes) - and need a handful of registers.  gfx950's lane
+// swaps exchange halves of two registers in one instruction; inside a row of 16 lanes the partners are mirrors (DPP).  Lane bit TOP tells b
+// from c, the three below it are n; lanes that differ in lower bits only hold shares of the same sum (TOP 32: xor 2 and 1, TOP 16: xor 1).
+template <int TOP, int LVL, int I, class F>
 __device__ __forceinline__ float pair_tree(F& f, int lane) {
     if constexpr (LVL == 0) {
         float b, c;
         f(Idx<I>{}, b, c);
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(b), __float_as_uint(c), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        return half_sum<TOP>(b, c, lane);
     } else {
-        const float lo = pair_tree<NP, LVL - 1, I>(f, lane), hi = pair_tree<NP, LVL - 1, I + (NP >> LVL)>(f, lane);
-        if constexpr (LVL == 1) {
-            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
-            return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-        }
-        if constexpr (LVL == 2) return ((lane & 8) ? hi : lo) + dpp_mirror((lane & 8) ? lo : hi);
-        if constexpr (LVL == 3) return ((lane & 4) ? hi : lo) + dpp_half_mirror((lane & 4) ? lo : hi);
-        if constexpr (LVL == 4) return ((lane & 2) ? hi : lo) + dpp_xor3((lane & 2) ? lo : hi);
-        if constexpr (LVL == 5) return ((lane & 1) ? hi : lo) + dpp_xor1((lane & 1) ? lo : hi);
+        const float lo = pair_tree<TOP, LVL - 1, I>(f, lane), hi = pair_tree<TOP, LVL - 1, I + (8 >> LVL)>(f, lane);
+        return half_sum<(TOP >> LVL)>(lo, hi, lane);
     }
-}
-template <int NP, class F>
-__device__ __forceinline__ float pair_sums(F& f, int lane) {
-    static_assert(NP == 8 || NP == 16 || NP == 32, "8, 16 or 32 pairs");
-    if constexpr (NP == 32) return pair_tree<32, 5, 0>(f, lane);
-    if constexpr (NP == 16) {
-        const float v = pair_tree<16, 4, 0>(f, lane);
-        return v + dpp_xor1(v);
-    }
-    float v = pair_tree<8, 3, 0>(f, lane);
-    v += dpp_xor3(v);
-    return v + dpp_xor1(v);
 }
 
 // The gradients of one network's weights: the partial sums [agent][slot][rows + extra][C] of its agents, in order.  The first `rows` rows go

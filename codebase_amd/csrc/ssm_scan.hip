@@ -2,13 +2,20 @@
 //
 //   h_t[n] = exp(dt_t A[n]) h_{t-1}[n] + dt_t B_t[n] x_t,   y_t = sum_n C_t[n] h_t[n] + D x_t        for every channel
 //
-// A wave owns 64 channels of one row and walks its steps with the state in registers; B and C of a step are the same for all of them and
-// come as LDS broadcasts.
+// Layout of a wave.  A lane keeps 8 states of one channel in registers, NS = 1, 2 or 4 lanes share a channel (N <= 8, 16, 32): lane =
+// group * CL + channel, CL = 64 / NS channels a wave.  The work of a step that does not depend on the state (loads, softplus, gate, store) is
+// done for NS steps at once, group g taking step s + g; a lane swap then hands every group the step it needs, and another one adds the groups'
+// shares of y.  So NS > 1 costs three swaps a step, keeps 8 / N of the registers and gives NS times the waves, which is what small batches need.
+// B and C of a step are the same for a group's channels and come as LDS broadcasts, K steps at a time.
 #include "ssm.h"
 
 using namespace marl;
 
 namespace {
+
+constexpr int K = 8;     // steps of a block: between two recorded states
+constexpr int NL = 8;    // states a lane keeps
+constexpr int WMAX = 8;  // waves of a backward workgroup
 
 struct ScanArgs {
     SsmDims d;
@@ -18,265 +25,553 @@ struct ScanArgs {
     const int32_t* lengths;
     void *y, *dx, *ddelta, *dB, *dC, *dz;
     float *h_out, *record, *dh_in;
-    float *pB, *pC;  // [nblk][P][S][B][G][N] partial sums of dB / dC, NULL: one block a group, written to dB / dC directly
+    float* carry;    // [row][chunk][N][C] states (forward) or gradients (backward) a chunk starts from; first its own contribution
+    float* sums;     // [row][chunk][C] sum of dt over a chunk, NaN with a reset inside
+    float *pB, *pC;  // [wgs][P][S][B][G][N] partial sums of dB / dC, NULL: one workgroup a row, which writes dB / dC
     float* part;     // [P][slots][N + 2][C] partial sums of dA, dD, ddelta_bias
-    int softplus, nblk, slots, nck;
-    int64_t items;
+    int softplus, nblk, slots, nck, chunk, nchunk, wpb, wgs;
+    int items;
 };
 
-// steps between two recorded states: their states of a block stay in registers in the backward pass (K * N of them)
-template <int NP>
-constexpr int scan_k() { return 128 / NP < 8 ? 4 : (NP == 8 ? 16 : 8); }
 inline int scan_np(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : 32); }
-inline int scan_k_of(int N) { return scan_np(N) == 8 ? scan_k<8>() : (scan_np(N) == 16 ? scan_k<16>() : scan_k<32>()); }
 
-// what a wave works on: 64 channels of one group, `bytes`-wise through row descriptors
-template <class T>
-struct ScanCols {
-    int g, kblk, first, nt, nf, vt, vf;  // group, block, first channel; bytes of a row of T / float; this lane's offsets
-    __device__ __forceinline__ ScanCols(const ScanArgs& a, int cb, int lane) {
+// ---- a wave's place ------------------------------------------------------------------------------------------------------------------
+template <class T, int NS>
+struct Lane {
+    static constexpr int CL = 64 / NS;
+    int lane, g, cl;      // group, channel within the block
+    int grp, kblk, first; // channel group, block within it, first channel
+    bool act;
+    int n0;               // first state
+    __device__ __forceinline__ Lane(const ScanArgs& a, int cb, int ln) {
         const int Cg = a.d.C / a.d.G;
-        g = cb / a.nblk;
-        kblk = cb % a.nblk;
-        first = g * Cg + kblk * 64;
-        const int left = (g + 1) * Cg - first, valid = left < 64 ? left : 64;
-        nt = valid * (int)sizeof(T);
-        nf = valid * 4;
-        vt = lane * (int)sizeof(T);
-        vf = lane * 4;
+        lane = ln;
+        g = ln / CL;
+        cl = ln % CL;
+        grp = uni(cb / a.nblk);
+        kblk = cb - grp * a.nblk;
+        first = grp * Cg + kblk * CL;
+        act = first + cl < (grp + 1) * Cg;
+        n0 = g * NL;
+    }
+    // offset of this lane's element of state n in an [N][C] array from its first channel
+    __device__ __forceinline__ int state_off(const ScanArgs& a, int n) const { return act && n0 + n < a.d.N ? ((n0 + n) * a.d.C + cl) * 4 : OOB; }
+    __device__ __forceinline__ int chan_off(int bytes) const { return act ? cl * bytes : OOB; }
+};
+
+template <class T, int NS>
+__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<T, NS>& q, const float* p, float scale, float (&r)[NL]) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first, p != nullptr ? ROW_MAX : 0, q.state_off(a, n));
+#pragma unroll
+    for (int n = 0; n < NL; ++n) r[n] *= scale;
+}
+template <class T, int NS>
+__device__ __forceinline__ void store_state(const ScanArgs& a, const Lane<T, NS>& q, float* p, const float (&r)[NL]) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) row_store(r[n], p + q.first, ROW_MAX, q.state_off(a, n));
+}
+
+// value of group i of a register that holds one value a group, in every group
+template <int NS>
+__device__ __forceinline__ void to_groups(float v, float (&r)[NS]) {
+    if constexpr (NS == 1) {
+        r[0] = v;
+    } else {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        if constexpr (NS == 2) {
+            r[0] = __uint_as_float(s[0]);
+            r[1] = __uint_as_float(s[1]);
+        } else {
+            const auto t = __builtin_amdgcn_permlane16_swap(s[0], s[0], false, false), u = __builtin_amdgcn_permlane16_swap(s[1], s[1], false, false);
+            r[0] = __uint_as_float(t[0]);
+            r[1] = __uint_as_float(t[1]);
+            r[2] = __uint_as_float(u[0]);
+            r[3] = __uint_as_float(u[1]);
+        }
+    }
+}
+// r[i]: every group's share for step i -> the sum for step g in group g
+template <int NS>
+__device__ __forceinline__ float from_groups(const float (&r)[NS]) {
+    if constexpr (NS == 1) return r[0];
+    if constexpr (NS == 2) return half_sum<32>(r[0], r[1], 0);
+    if constexpr (NS == 4) return half_sum<16>(half_sum<32>(r[0], r[2], 0), half_sum<32>(r[1], r[3], 0), 0);
+}
+
+// ---- K steps of inputs, requested ahead of their use ----------------------------------------------------------------------------------------
+template <class T>
+struct Raw;  // an element as it comes, widened at its use
+template <>
+struct Raw<float> {
+    float v;
+    __device__ __forceinline__ float get() const { return v; }
+    __device__ __forceinline__ void load(const float* p, int voff) { v = row_load(p, ROW_MAX, voff); }
+};
+template <class T>
+struct Raw {
+    unsigned short v;
+    __device__ __forceinline__ float get() const { return up(__builtin_bit_cast(T, v)); }
+    __device__ __forceinline__ void load(const T* p, int voff) { v = __builtin_amdgcn_raw_buffer_load_b16(row_rsrc(p, ROW_MAX), voff, 0, 0); }
+};
+
+// offset of step t0 + i NS + g of a sequence from step t0 + i NS; steps from `end` on are not there
+template <class T, int NS>
+struct SeqPtr {
+    const T* p;
+    int64_t st;
+    int voff;
+    __device__ __forceinline__ SeqPtr(const SsmSeq& s, const Lane<T, NS>& q, int pa, int b)
+        : p(seq_at<T>(s, pa, b) + q.first), st(s.st), voff(q.act ? q.g * (int)(s.st * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB) {}
+    __device__ __forceinline__ void load(Raw<T>& r, int64_t t, int out) const { r.load(p + t * st, voff | out); }
+};
+// -1's sign bit where step t + g is behind the end: OR-ed into an offset it points behind any row
+__device__ __forceinline__ int behind(int t, int g, int end) { return (end - 1 - t - g) & OOB; }
+
+// B / C of K steps: what this thread of NT carries to LDS
+template <class T, int NP, int NT>
+struct Maps {
+    static constexpr int M = (K * NP + NT - 1) / NT;
+    Raw<T> b[M], c[M];
+    __device__ __forceinline__ void load(const ScanArgs& a, const T* Bp, const T* Cp, int t0, int end, int tid) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int e = tid + NT * i, s = e / NP, n = e % NP;
+            const bool ok = e < K * NP && n < a.d.N && t0 + s < end;
+            const int64_t t = ok ? t0 + s : t0, m = ok ? n : 0;
+            b[i].v = reinterpret_cast<const decltype(b[i].v)*>(Bp)[t * a.Bm.st + m];
+            c[i].v = reinterpret_cast<const decltype(c[i].v)*>(Cp)[t * a.Cm.st + m];
+            if (!ok) b[i].v = 0, c[i].v = 0;
+        }
+    }
+    __device__ __forceinline__ void store(float* lb, float* lc, int tid) const {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int e = tid + NT * i;
+            if (NT * M == K * NP || e < K * NP) {
+                lb[e] = b[i].get();
+                lc[e] = c[i].get();
+            }
+        }
     }
 };
 
-// B and C of K steps from t0 on (zeros behind the end and in the padding up to NP) to the wave's LDS, f32
-template <class T, int NP, int K>
-__device__ __forceinline__ void stage_maps(const ScanArgs& a, const T* Bp, const T* Cp, int t0, int len, float* lb, float* lc, int lane) {
-#pragma unroll
-    for (int i = 0; i < (K * NP + 63) / 64; ++i) {
-        const int e = lane + 64 * i, s = e / NP, n = e % NP, t = t0 + s;
-        if (K * NP >= 64 || e < K * NP) {
-            const bool ok = n < a.d.N && t < len;
-            lb[e] = ok ? up(Bp[t * a.Bm.st + n]) : 0.f;
-            lc[e] = ok ? up(Cp[t * a.Cm.st + n]) : 0.f;
-        }
-    }
+// bit s: an episode starts at step t0 + s
+__device__ __forceinline__ int load_reset(const ScanArgs& a, int b, int t0, int end, int lane) {
+    if (a.reset == nullptr) return 0;
+    const int t = t0 + (lane % K);
+    return t < end ? a.reset[(int64_t)t * a.d.B + b] : 0;
+}
+__device__ __forceinline__ unsigned reset_bits(int v) { return (unsigned)__builtin_amdgcn_ballot_w64(v != 0) & ((1u << K) - 1); }
+
+__device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bias) {
+    const float r = d + bias;
+    return a.softplus ? softplus(r) : r;
 }
 
-template <class T, int NP>
+// ---- forward ---------------------------------------------------------------------------------------------------------------------------
+// CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass)
+template <class T, int NS, bool CARRY>
 __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
-    constexpr int K = scan_k<NP>();
+    constexpr int NP = NS * NL, KG = K / NS;
     __shared__ float lds[4][2][K * NP];
-    const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
-    const int64_t item = (int64_t)blockIdx.x * 4 + wv;
+    const int wv = uni(threadIdx.x >> 6);
+    const int item = blockIdx.x * 4 + wv;
     if (item >= a.items) return;
-    const int N = a.d.N, C = a.d.C, S = a.d.S, ncb = a.d.G * a.nblk;
-    const int cb = (int)(item % ncb), row = (int)(item / ncb), p = row / a.d.B, b = row % a.d.B;
-    const ScanCols<T> q(a, cb, lane);
-    const int net = a.d.net[p], len = uni(seq_len(a.lengths, b, S));
-    float A[NP], h[NP];
+    const int ncb = a.d.G * a.nblk, rc = uni(item / ncb), cb = item - rc * ncb;  // rc: (row, chunk)
+    const int row = uni(rc / a.nchunk), ch = rc - row * a.nchunk, p = uni(row / a.d.B), b = row - p * a.d.B;
+    const Lane<T, NS> q(a, cb, threadIdx.x & 63);
+    const int N = a.d.N, C = a.d.C, net = a.d.net[p], len = uni(seq_len(a.lengths, b, a.d.S));
+    const int first = ch * a.chunk, last = first + a.chunk < a.d.S ? first + a.chunk : a.d.S, end = len < last ? len : last;
+    const SeqPtr<T, NS> xs(a.x, q, p, b), ds(a.delta, q, p, b), zs(a.z, q, p, b);
+    const T *Bp = seq_at<T>(a.Bm, p, b) + q.grp * N, *Cp = seq_at<T>(a.Cm, p, b) + q.grp * N;
+    const bool gated = !CARRY && a.z.data != nullptr;
+    const int lane = q.lane;
+
+    Raw<T> x[KG], dr[KG], z[KG];
+    Maps<T, NP, 64> maps;
+    int rs;
+    auto request = [&](int t0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-        A[n] = n < N ? row_load(a.A + ((int64_t)net * N + n) * C + q.first, q.nf, q.vf) * LOG2E : 0.f;
-        h[n] = n < N && a.h_in != nullptr ? row_load(a.h_in + ((int64_t)row * N + n) * C + q.first, q.nf, q.vf) : 0.f;
-    }
-    const float D = a.D != nullptr ? row_load(a.D + (int64_t)net * C + q.first, q.nf, q.vf) : 0.f;
-    const float bias = a.bias != nullptr ? row_load(a.bias + (int64_t)net * C + q.first, q.nf, q.vf) : 0.f;
-    const T *xp = seq_at<T>(a.x, p, b) + q.first, *dp = seq_at<T>(a.delta, p, b) + q.first, *zp = seq_at<T>(a.z, p, b) + q.first;
-    const T *Bp = seq_at<T>(a.Bm, p, b) + q.g * N, *Cp = seq_at<T>(a.Cm, p, b) + q.g * N;
-    T* yp = static_cast<T*>(a.y) + ((int64_t)p * S * a.d.B + b) * C + q.first;
+        for (int i = 0; i < KG; ++i) {
+            const int out = behind(t0 + i * NS, q.g, end);
+            xs.load(x[i], t0 + i * NS, out);
+            ds.load(dr[i], t0 + i * NS, out);
+            if (gated) zs.load(z[i], t0 + i * NS, out);
+        }
+        maps.load(a, Bp, Cp, t0, end, lane);
+        rs = load_reset(a, b, t0, end, lane);
+    };
+    if (first < end) request(first);
+    float A[NL], h[NL];
+    load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
+    if (CARRY) load_state(a, q, (const float*)nullptr, 1.f, h);
+    else load_state(a, q, a.nchunk > 1 ? a.carry + ((int64_t)row * a.nchunk + ch) * N * C : (a.h_in != nullptr ? a.h_in + (int64_t)row * N * C : nullptr), 1.f, h);
+    const int co = q.chan_off(4);
+    const float D = row_load(a.D + (int64_t)net * C + q.first, a.D != nullptr ? ROW_MAX : 0, co);
+    const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, co);
+    T* yp = static_cast<T*>(a.y) + ((int64_t)p * a.d.S * a.d.B + b) * C + q.first;
     const int64_t yst = (int64_t)a.d.B * C;
-    const bool gated = a.z.data != nullptr;
+    const int yoff = q.act ? q.g * (int)(yst * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB;
     float *lb = lds[wv][0], *lc = lds[wv][1];
-    for (int t0 = 0; t0 < len; t0 += K) {
+    float total = 0.f;  // CARRY: sum of dt
+    for (int t0 = first; t0 < end; t0 += K) {
         wave_lds_sync();
-        stage_maps<T, NP, K>(a, Bp, Cp, t0, len, lb, lc, lane);
-        if (a.record != nullptr)
+        maps.store(lb, lc, lane);
+        const unsigned fresh = reset_bits(rs);
+        float xv[KG], dt[KG], gate[KG];
 #pragma unroll
-            for (int n = 0; n < NP; ++n)
-                if (n < N) row_store(h[n], a.record + (((int64_t)row * a.nck + t0 / K) * N + n) * C + q.first, q.nf, q.vf);
+        for (int i = 0; i < KG; ++i) {
+            xv[i] = x[i].get();
+            dt[i] = step_size(a, dr[i].get(), bias);
+            gate[i] = gated ? z[i].get() : 0.f;
+        }
         wave_lds_sync();
-        const int m = len - t0 < K ? len - t0 : K;
-        for (int s = 0; s < m; ++s) {
-            const int64_t t = t0 + s;
-            const float x = row_load(xp + t * a.x.st, q.nt, q.vt), dr = row_load(dp + t * a.delta.st, q.nt, q.vt) + bias;
-            const float z = gated ? row_load(zp + t * a.z.st, q.nt, q.vt) : 0.f;
-            const float dt = a.softplus ? softplus(dr) : dr, u = dt * x;
-            if (a.reset != nullptr && a.reset[t * a.d.B + b] != 0)
+        if (t0 + K < end) request(t0 + K);
+        if (!CARRY && a.record != nullptr) store_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, h);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) h[n] = 0.f;
-            float y = D * x;
+        for (int i = 0; i < KG; ++i) {
+            if (t0 + i * NS >= end) break;
+            const int out = behind(t0 + i * NS, q.g, end);
+            const float dti = out ? 0.f : dt[i];
+            float dts[NS], us[NS], ys[NS];
+            to_groups<NS>(dti, dts);
+            to_groups<NS>(dti * xv[i], us);
+            if (CARRY) total += fresh >> (i * NS + q.g) & 1 ? __builtin_nanf("") : dti;
 #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                h[n] = fmaf(exp2_fast(dt * A[n]), h[n], u * lb[s * NP + n]);
-                y = fmaf(h[n], lc[s * NP + n], y);
+            for (int j = 0; j < NS; ++j) {
+                const int s = i * NS + j;
+                if (fresh >> s & 1)
+#pragma unroll
+                    for (int n = 0; n < NL; ++n) h[n] = 0.f;
+                float y = 0.f;
+#pragma unroll
+                for (int n = 0; n < NL; ++n) {
+                    h[n] = fmaf(exp2_fast(dts[j] * A[n]), h[n], us[j] * lb[s * NP + q.n0 + n]);
+                    if (!CARRY) y = fmaf(h[n], lc[s * NP + q.n0 + n], y);
+                }
+                ys[j] = y;
             }
-            if (gated) y *= z * sigmoid(z);
-            row_store(y, yp + t * yst, q.nt, q.vt);
+            if (!CARRY) {
+                float y = fmaf(D, xv[i], from_groups<NS>(ys));
+                if (gated) y *= gate[i] * sigmoid(gate[i]);
+                row_store(y, yp + (t0 + i * NS) * yst, ROW_MAX, yoff | out);
+            }
         }
     }
-    for (int t = len; t < S; ++t) row_store(0.f, yp + t * yst, q.nt, q.vt);
-    if (a.h_out != nullptr)
+    if (CARRY) {
+        store_state(a, q, a.carry + ((int64_t)row * a.nchunk + ch) * N * C, h);
+        float r[NS];
+        to_groups<NS>(total, r);
+        total = r[0];
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
-            if (n < N) row_store(h[n], a.h_out + ((int64_t)row * N + n) * C + q.first, q.nf, q.vf);
+        for (int j = 1; j < NS; ++j) total += r[j];
+        row_store(total, a.sums + ((int64_t)row * a.nchunk + ch) * C + q.first, ROW_MAX, q.g == 0 ? co : OOB);
+        return;
+    }
+    for (int t = end > first ? end : first; t < last; ++t) row_store(0.f, yp + t * yst, ROW_MAX, q.g == 0 ? q.chan_off(sizeof(T)) : OOB);
+    if (a.h_out != nullptr && ch == a.nchunk - 1) store_state(a, q, a.h_out + (int64_t)row * N * C, h);
 }
 
-// Backward: blocks of K steps from the last to the first; a block's states are recomputed from its record into registers, then the steps
-// run backwards with G_t = C_t dys_t + exp(dt_{t+1} A) G_{t+1} (dys: dy through the gate).
-template <class T, int NP>
-__global__ __launch_bounds__(256, NP == 32 ? 1 : 2) void ssm_scan_bwd_kernel(ScanArgs a) {
-    constexpr int K = scan_k<NP>();
-    __shared__ float lds[4][2][K * NP];
-    const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
-    const int64_t item = (int64_t)blockIdx.x * 4 + wv;
-    if (item >= a.items) return;
-    const int N = a.d.N, C = a.d.C, S = a.d.S, NB = a.d.B, ncb = a.d.G * a.nblk;
-    const int cb = (int)(item % ncb), ps = (int)(item / ncb), p = ps / a.slots, slot = ps % a.slots;
-    const ScanCols<T> q(a, cb, lane);
-    const int net = a.d.net[p];
-    float A[NP], dA[NP];
-#pragma unroll
-    for (int n = 0; n < NP; ++n) {
-        A[n] = n < N ? row_load(a.A + ((int64_t)net * N + n) * C + q.first, q.nf, q.vf) * LOG2E : 0.f;
-        dA[n] = 0.f;
+// Joins the chunks of a sequence: carry[j] (what chunk j contributes) becomes what chunk j starts from.  A chunk multiplies what it is given by
+// exp(A sum dt), or drops it at a reset (sum = NaN).  A workgroup takes 64 channels of one state, its 16 waves a run of chunks each; the runs
+// are joined through LDS, so the serial part is nchunk / 16 steps twice and 16 once.  reverse: from the last chunk to the first.
+__global__ __launch_bounds__(1024) void ssm_scan_join_kernel(ScanArgs a, const float* __restrict__ start, int reverse) {
+    __shared__ float ls[16][64], lh[16][64];
+    const int cbs = (a.d.C + 63) / 64, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int n = (blockIdx.x / cbs) % a.d.N, row = blockIdx.x / cbs / a.d.N, c0 = (blockIdx.x % cbs) * 64 + lane;
+    const bool act = c0 < a.d.C;
+    const int c = act ? c0 : a.d.C - 1;
+    const float A = a.A[((int64_t)a.d.net[row / a.d.B] * a.d.N + n) * a.d.C + c] * LOG2E;
+    const int per = (a.nchunk + 15) / 16, lo = w * per, hi = lo + per < a.nchunk ? lo + per : a.nchunk;
+    auto at = [&](int k) { return (int64_t)row * a.nchunk + (reverse ? a.nchunk - 1 - k : k); };
+    auto apply = [&](float s, float own, float h) { return s == s ? fmaf(exp2_fast(A * s), h, own) : own; };
+    float s = 0.f, h = 0.f;
+#pragma unroll 4
+    for (int k = lo; k < hi; ++k) {
+        const float sk = a.sums[at(k) * a.d.C + c], own = a.carry[(at(k) * a.d.N + n) * a.d.C + c];
+        h = apply(sk, own, h);
+        s += sk;
     }
-    const float D = a.D != nullptr ? row_load(a.D + (int64_t)net * C + q.first, q.nf, q.vf) : 0.f;
-    const float bias = a.bias != nullptr ? row_load(a.bias + (int64_t)net * C + q.first, q.nf, q.vf) : 0.f;
-    float dD = 0.f, dbias = 0.f;
-    float *lb = lds[wv][0], *lc = lds[wv][1];
-    const int64_t yst = (int64_t)NB * C;
-    const int64_t mst = (int64_t)NB * a.d.G * N;  // between steps of dB / dC
-    // the lane's place in a row of dB or dC (lanes with nothing to store point behind the row): pair_sums leaves b_n at lane n R, c_n behind
-    constexpr int R = 32 / NP;
-    const int mi = lane / R, mn = mi % NP;
-    const bool mine = lane % R == 0 && mn < N;
-    const int me = a.pB != nullptr ? 4 : (int)sizeof(T);
-    const int vB = mine && mi < NP ? mn * me : 1 << 30, vC = mine && mi >= NP ? mn * me : 1 << 30;
+    ls[w][lane] = s;
+    lh[w][lane] = h;
+    __syncthreads();
+    h = start != nullptr ? start[((int64_t)row * a.d.N + n) * a.d.C + c] : 0.f;
+    for (int k = 0; k < w; ++k) h = apply(ls[k][lane], lh[k][lane], h);
+#pragma unroll 4
+    for (int k = lo; k < hi; ++k) {
+        float* q = a.carry + (at(k) * a.d.N + n) * a.d.C + c;
+        const float sk = a.sums[at(k) * a.d.C + c], own = *q;
+        if (act) *q = h;
+        h = apply(sk, own, h);
+    }
+}
+
+// ---- backward --------------------------------------------------------------------------------------------------------------------------
+// G_t = C_t dys_t + exp(dt_{t+1} A) G_{t+1} (dys: dy through the gate); a chunk leaves exp(dt_t A) G_t of its first step.
+// CARRY pass of a split sequence: what a chunk leaves by itself, and its sum of dt.
+template <class T, int NS>
+__global__ __launch_bounds__(256) void ssm_scan_bwd_carry_kernel(ScanArgs a) {
+    constexpr int NP = NS * NL, KG = K / NS;
+    __shared__ float lds[4][2][K * NP];
+    const int wv = uni(threadIdx.x >> 6);
+    const int item = blockIdx.x * 4 + wv;
+    if (item >= a.items) return;
+    const int ncb = a.d.G * a.nblk, rc = uni(item / ncb), cb = item - rc * ncb;
+    const int row = uni(rc / a.nchunk), ch = rc - row * a.nchunk, p = uni(row / a.d.B), b = row - p * a.d.B;
+    const Lane<T, NS> q(a, cb, threadIdx.x & 63);
+    const int N = a.d.N, C = a.d.C, net = a.d.net[p], len = uni(seq_len(a.lengths, b, a.d.S)), lane = q.lane;
+    const int first = ch * a.chunk, last = first + a.chunk < a.d.S ? first + a.chunk : a.d.S, end = len < last ? len : last;
+    const SeqPtr<T, NS> ds(a.delta, q, p, b), zs(a.z, q, p, b), gs(a.dy, q, p, b);
+    const T* Cp = seq_at<T>(a.Cm, p, b) + q.grp * N;
     const bool gated = a.z.data != nullptr;
-    for (int b = slot; b < NB; b += a.slots) {
-        const int row = p * NB + b, len = uni(seq_len(a.lengths, b, S));
-        const T *xp = seq_at<T>(a.x, p, b) + q.first, *dp = seq_at<T>(a.delta, p, b) + q.first, *zp = seq_at<T>(a.z, p, b) + q.first;
-        const T *Bp = seq_at<T>(a.Bm, p, b) + q.g * N, *Cp = seq_at<T>(a.Cm, p, b) + q.g * N, *gp = seq_at<T>(a.dy, p, b) + q.first;
-        const int64_t o = ((int64_t)p * S * NB + b) * C + q.first, om = (((int64_t)p * S * NB + b) * a.d.G + q.g) * N;
-        const int64_t pm = om + (int64_t)q.kblk * a.d.P * S * NB * a.d.G * N;
-        T *dxp = static_cast<T*>(a.dx) + o, *ddp = static_cast<T*>(a.ddelta) + o, *dzp = static_cast<T*>(a.dz) + o;
-        auto put_maps = [&](float v, int64_t t, bool in) {
-            const int n = in ? N * me : 0;
-            if (a.pB != nullptr) {
-                row_store(v, a.pB + pm + t * mst, n, vB);
-                row_store(v, a.pC + pm + t * mst, n, vC);
-            } else {
-                row_store(v, static_cast<T*>(a.dB) + om + t * mst, n, vB);
-                row_store(v, static_cast<T*>(a.dC) + om + t * mst, n, vC);
-            }
-        };
-        float dh[NP];
+    float A[NL], dh[NL];
+    load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
+    load_state(a, q, (const float*)nullptr, 1.f, dh);
+    const int co = q.chan_off(4);
+    const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, co);
+    float *lb = lds[wv][0], *lc = lds[wv][1];
+    float total = 0.f;
+    Raw<T> dr[KG], z[KG], gy[KG];
+    Maps<T, NP, 64> maps;
+    int rs;
+    auto request = [&](int t0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
-            dh[n] = n < N && a.dh_out != nullptr ? row_load(a.dh_out + ((int64_t)row * N + n) * C + q.first, q.nf, q.vf) : 0.f;
-        for (int t = S - 1; t >= len; --t) {  // behind the end
-            row_store(0.f, dxp + t * yst, q.nt, q.vt);
-            row_store(0.f, ddp + t * yst, q.nt, q.vt);
-            if (gated) row_store(0.f, dzp + t * yst, q.nt, q.vt);
-            put_maps(0.f, t, true);
+        for (int i = 0; i < KG; ++i) {
+            const int out = behind(t0 + i * NS, q.g, end);
+            ds.load(dr[i], t0 + i * NS, out);
+            gs.load(gy[i], t0 + i * NS, out);
+            if (gated) zs.load(z[i], t0 + i * NS, out);
         }
-        for (int t0 = (len - 1) / K * K; t0 >= 0 && len > 0; t0 -= K) {
-            wave_lds_sync();
-            stage_maps<T, NP, K>(a, Bp, Cp, t0, len, lb, lc, lane);
-            wave_lds_sync();
-            float hs[K + 1][NP];  // hs[s]: the state before step s; hs[K]: after the block
+        maps.load(a, Cp, Cp, t0, end, lane);
+        rs = load_reset(a, b, t0, end, lane);
+    };
+    const int tl = first + (end - 1 - first) / K * K;
+    if (first < end) request(tl);
+    for (int t0 = tl; t0 >= first && first < end; t0 -= K) {
+        wave_lds_sync();
+        maps.store(lb, lc, lane);
+        const unsigned fresh = reset_bits(rs);
+        float dt[KG], dys[KG];
 #pragma unroll
-            for (int n = 0; n < NP; ++n)
-                hs[0][n] = n < N ? row_load(a.record + (((int64_t)row * a.nck + t0 / K) * N + n) * C + q.first, q.nf, q.vf) : 0.f;
-            float x[K], dr[K], dt[K], dys[K], zv[K];
-            unsigned fresh = 0;
-#pragma unroll
-            for (int s = 0; s < K; ++s) {
-                const int64_t t = t0 + s;
-                const bool in = t < len;  // a step behind the end changes nothing: dt = 0, x = 0, dy = 0
-                const int nt = in ? q.nt : 0;
-                x[s] = row_load(xp + t * a.x.st, nt, q.vt);
-                dr[s] = row_load(dp + t * a.delta.st, nt, q.vt) + bias;
-                dys[s] = row_load(gp + t * a.dy.st, nt, q.vt);
-                zv[s] = gated ? row_load(zp + t * a.z.st, nt, q.vt) : 0.f;
-                if (in && a.reset != nullptr && a.reset[t * NB + b] != 0) fresh |= 1u << s;
-                __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < KG; ++i) {
+            dt[i] = behind(t0 + i * NS, q.g, end) ? 0.f : step_size(a, dr[i].get(), bias);
+            dys[i] = gy[i].get();
+            if (gated) {
+                const float v = z[i].get();
+                dys[i] *= v * sigmoid(v);
             }
+        }
+        wave_lds_sync();
+        if (t0 > first) request(t0 - K);
 #pragma unroll
-            for (int s = 0; s < K; ++s) {
-                const int64_t t = t0 + s;
-                const bool in = t < len;
-                dt[s] = in ? (a.softplus ? softplus(dr[s]) : dr[s]) : 0.f;
-                const float u = dt[s] * x[s];
-                // a reset empties the state through the decay, e^-inf = 0; what is not finite has to go by hand
-                const bool re = fresh >> s & 1;
-                const float fr = re ? -INFINITY : 0.f;
-                if (re)
+        for (int i = KG - 1; i >= 0; --i) {
+            float dts[NS], gys[NS];
+            to_groups<NS>(dt[i], dts);
+            to_groups<NS>(dys[i], gys);
+            total += fresh >> (i * NS + q.g) & 1 ? __builtin_nanf("") : dt[i];
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) hs[s][n] = fabsf(hs[s][n]) < INFINITY ? hs[s][n] : 0.f;
-                float y = D * x[s];
+            for (int j = NS - 1; j >= 0; --j) {
+                const int s = i * NS + j;
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    hs[s + 1][n] = fmaf(exp2_fast(fmaf(dt[s], A[n], fr)), hs[s][n], u * lb[s * NP + n]);
-                    y = fmaf(hs[s + 1][n], lc[s * NP + n], y);
+                for (int n = 0; n < NL; ++n) dh[n] = fmaf(gys[j], lc[s * NP + q.n0 + n], dh[n]) * exp2_fast(dts[j] * A[n]);
+                if (fresh >> s & 1)
+#pragma unroll
+                    for (int n = 0; n < NL; ++n) dh[n] = 0.f;
+            }
+        }
+    }
+    store_state(a, q, a.carry + ((int64_t)row * a.nchunk + ch) * N * C, dh);
+    float r[NS];
+    to_groups<NS>(total, r);
+    total = r[0];
+#pragma unroll
+    for (int j = 1; j < NS; ++j) total += r[j];
+    row_store(total, a.sums + ((int64_t)row * a.nchunk + ch) * C + q.first, ROW_MAX, q.g == 0 ? co : OOB);
+}
+
+// value i of a step's row of maps (i < NP: dB, else dC)
+template <class T, int NP>
+__device__ __forceinline__ void put_map(const ScanArgs& a, float v, int64_t om, int64_t pm, int64_t at, int i) {
+    const int n = i % NP;
+    if (n >= a.d.N) return;
+    if (a.pB != nullptr) (i < NP ? a.pB : a.pC)[pm + at + n] = v;
+    else static_cast<T*>(i < NP ? a.dB : a.dC)[om + at + n] = down<T>(v);
+}
+
+// Blocks of K steps from the last to the first: a block's states are recomputed from its record into registers, then its steps run backwards.
+// A workgroup's waves own neighbouring channels of the same rows: they share B and C in LDS and add up their shares of dB and dC there.
+template <class T, int NS>
+__global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) {
+    constexpr int NP = NS * NL, KG = K / NS, TOP = 32 / NS;
+    __shared__ float lb[K * NP], lc[K * NP], red[WMAX][K][2 * NP];
+    const int wv = uni(threadIdx.x >> 6), nthr = a.wpb * 64;
+    // workgroup -> (agent, slot, channel group, run of blocks)
+    const int gw = a.d.G * a.wgs, ps = uni((int)blockIdx.x / gw), wg = (int)blockIdx.x - ps * gw, p = uni(ps / a.slots), slot = ps - p * a.slots;
+    const int grp = uni(wg / a.wgs), run = wg - grp * a.wgs;
+    const int kblk = run * a.wpb + wv;  // may lie behind the last block: such a wave has no channels and only helps along
+    Lane<T, NS> q(a, grp * a.nblk + (kblk < a.nblk ? kblk : a.nblk - 1), threadIdx.x & 63);
+    if (kblk >= a.nblk) q.act = false;
+    const int N = a.d.N, C = a.d.C, S = a.d.S, NB = a.d.B, net = a.d.net[p], lane = q.lane;
+    float A[NL], dA[NL];
+    load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
+#pragma unroll
+    for (int n = 0; n < NL; ++n) dA[n] = 0.f;
+    const int co = q.chan_off(4);
+    const float D = row_load(a.D + (int64_t)net * C + q.first, a.D != nullptr ? ROW_MAX : 0, co);
+    const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, co);
+    float dD = 0.f, dbias = 0.f;
+    const int64_t yst = (int64_t)NB * C, mst = (int64_t)NB * a.d.G * N;
+    const int yoff = q.act ? q.g * (int)(yst * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB;
+    const bool gated = a.z.data != nullptr;
+    for (int it = slot; it < NB * a.nchunk; it += a.slots) {
+        const int b = uni(it / a.nchunk), ch = it - b * a.nchunk;
+        const int row = p * NB + b, len = uni(seq_len(a.lengths, b, S));
+        const int first = ch * a.chunk, last = first + a.chunk < S ? first + a.chunk : S, end = len < last ? len : last;
+        const SeqPtr<T, NS> xs(a.x, q, p, b), ds(a.delta, q, p, b), zs(a.z, q, p, b), gs(a.dy, q, p, b);
+        const T *Bp = seq_at<T>(a.Bm, p, b) + grp * N, *Cp = seq_at<T>(a.Cm, p, b) + grp * N;
+        const int64_t o = ((int64_t)p * S * NB + b) * C + q.first, om = (((int64_t)p * S * NB + b) * a.d.G + grp) * N;
+        const int64_t pm = om + (int64_t)run * a.d.P * S * NB * a.d.G * N;
+        T *dxp = static_cast<T*>(a.dx) + o, *ddp = static_cast<T*>(a.ddelta) + o, *dzp = static_cast<T*>(a.dz) + o;
+        float dh[NL];
+        load_state(a, q, a.nchunk > 1 ? a.carry + ((int64_t)row * a.nchunk + ch) * N * C : (a.dh_out != nullptr ? a.dh_out + (int64_t)row * N * C : nullptr), 1.f, dh);
+        for (int t = last - 1; t >= end && t >= first; --t) {  // behind the end
+            const int off = q.g == 0 ? q.chan_off(sizeof(T)) : OOB;
+            row_store(0.f, dxp + t * yst, ROW_MAX, off);
+            row_store(0.f, ddp + t * yst, ROW_MAX, off);
+            if (gated) row_store(0.f, dzp + t * yst, ROW_MAX, off);
+            for (int i = threadIdx.x; i < 2 * NP; i += nthr) put_map<T, NP>(a, 0.f, om, pm, t * mst, i);
+        }
+        for (int t0 = first + (end - 1 - first) / K * K; t0 >= first && first < end; t0 -= K) {
+            Raw<T> xr[KG], dr[KG], zr[KG], gr[KG];
+            Maps<T, NP, 64> maps;
+#pragma unroll
+            for (int i = 0; i < KG; ++i) {
+                const int out = behind(t0 + i * NS, q.g, end);
+                xs.load(xr[i], t0 + i * NS, out);
+                ds.load(dr[i], t0 + i * NS, out);
+                gs.load(gr[i], t0 + i * NS, out);
+                if (gated) zs.load(zr[i], t0 + i * NS, out);
+            }
+            const int rs = load_reset(a, b, t0, end, lane);
+            float hs[K + 1][NL];  // hs[s]: the state before step s; hs[K]: after the block
+            load_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, 1.f, hs[0]);
+            if (wv == 0) {
+                maps.load(a, Bp, Cp, t0, end, lane);
+                maps.store(lb, lc, lane);
+            }
+            __syncthreads();
+            const unsigned fresh = reset_bits(rs);
+            float x[KG], dt[KG], dys[KG], sd[KG];  // sd: the step size's slope
+#pragma unroll
+            for (int i = 0; i < KG; ++i) {
+                const int out = behind(t0 + i * NS, q.g, end);  // a step behind the end changes nothing: dt = 0, x = 0, dy = 0
+                const float raw = dr[i].get() + bias;
+                x[i] = xr[i].get();
+                dt[i] = out ? 0.f : (a.softplus ? softplus(raw) : raw);
+                sd[i] = a.softplus ? sigmoid(raw) : 1.f;
+                float dts[NS], us[NS], ys[NS];
+                to_groups<NS>(dt[i], dts);
+                to_groups<NS>(dt[i] * x[i], us);
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    const int s = i * NS + j;
+                    // a reset empties the state through the decay, e^-inf = 0; what is not finite has to go by hand
+                    const bool re = fresh >> s & 1;
+                    const float fr = re ? -INFINITY : 0.f;
+                    if (re)
+#pragma unroll
+                        for (int n = 0; n < NL; ++n) hs[s][n] = fabsf(hs[s][n]) < INFINITY ? hs[s][n] : 0.f;
+                    float y = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NL; ++n) {
+                        hs[s + 1][n] = fmaf(exp2_fast(fmaf(dts[j], A[n], fr)), hs[s][n], us[j] * lb[s * NP + q.n0 + n]);
+                        y = fmaf(hs[s + 1][n], lc[s * NP + q.n0 + n], y);
+                    }
+                    ys[j] = y;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                dys[i] = gr[i].get();
                 if (gated) {
-                    const float sg = sigmoid(zv[s]);
-                    row_store(dys[s] * y * sg * fmaf(zv[s], 1.f - sg, 1.f), dzp + t * yst, in ? q.nt : 0, q.vt);
-                    dys[s] *= zv[s] * sg;
+                    const float y = fmaf(D, x[i], from_groups<NS>(ys)), z = zr[i].get(), sg = sigmoid(z);
+                    row_store(dys[i] * y * sg * fmaf(z, 1.f - sg, 1.f), dzp + (t0 + i * NS) * yst, ROW_MAX, yoff | out);
+                    dys[i] *= z * sg;
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
             // below, addresses, maps and decays are formed anew: kept from above they would cost more registers than they save time
-            int t1 = t0;
+            int t1 = uni(t0);
             asm volatile("" : "+s"(t1)::"memory");
 #pragma unroll
-            for (int s = K - 1; s >= 0; --s) {
-                asm volatile("" : "+v"(dt[s])::"memory");
-                const int64_t t = t1 + s;
-                const bool in = t < len;
-                const bool re = fresh >> s & 1;
-                const float fr = re ? -INFINITY : 0.f, u = dt[s] * x[s];
-                float gb = 0.f, ga = 0.f;
-                auto state = [&](auto idx, float& vb, float& vc) {
-                    constexpr int n = decltype(idx)::v;
-                    vc = dys[s] * hs[s + 1][n];  // dC
-                    const float gn = fmaf(dys[s], lc[s * NP + n], dh[n]);
-                    vb = gn * u;                 // dB
-                    gb = fmaf(gn, lb[s * NP + n], gb);
-                    dh[n] = gn * exp2_fast(fmaf(dt[s], A[n], fr));
-                    const float w = dh[n] * hs[s][n];
-                    ga = fmaf(w, A[n], ga);
-                    dA[n] = fmaf(w, dt[s], dA[n]);
-                };
-                const float sum = pair_sums<NP>(state, lane);
-                if (re)
+            for (int i = KG - 1; i >= 0; --i) {
+                asm volatile("" : "+v"(dt[i])::"memory");
+                float dts[NS], us[NS], gys[NS], gb[NS], ga[NS];
+                to_groups<NS>(dt[i], dts);
+                to_groups<NS>(dt[i] * x[i], us);
+                to_groups<NS>(dys[i], gys);
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) dh[n] = 0.f;
-                dD = fmaf(dys[s], x[s], dD);
-                float dd = fmaf(LN2, ga, gb * x[s]);
-                if (a.softplus) dd *= sigmoid(dr[s]);
-                if (!in) dd = 0.f;
+                for (int j = NS - 1; j >= 0; --j) {
+                    const int s = i * NS + j;
+                    const bool re = fresh >> s & 1;
+                    const float fr = re ? -INFINITY : 0.f;
+                    float sb = 0.f, sa = 0.f;
+                    auto state = [&](auto idx, float& vb, float& vc) __attribute__((always_inline)) {
+                        constexpr int n = decltype(idx)::v;
+                        vc = gys[j] * hs[s + 1][n];  // dC
+                        const float gn = fmaf(gys[j], lc[s * NP + q.n0 + n], dh[n]);
+                        vb = gn * us[j];             // dB
+                        sb = fmaf(gn, lb[s * NP + q.n0 + n], sb);
+                        dh[n] = gn * exp2_fast(fmaf(dts[j], A[n], fr));
+                        const float w = dh[n] * hs[s][n];
+                        sa = fmaf(w, A[n], sa);
+                        dA[n] = fmaf(w, dts[j], dA[n]);
+                    };
+                    float sum = pair_tree<TOP, 3, 0>(state, lane);
+                    if constexpr (NS == 1) sum += dpp_xor3(sum);
+                    if constexpr (NS <= 2) sum += dpp_xor1(sum);
+                    gb[j] = sb;
+                    ga[j] = sa;
+                    if (re)
+#pragma unroll
+                        for (int n = 0; n < NL; ++n) dh[n] = 0.f;
+                    // lane bit TOP: dB / dC, the three below: n (within the lane's group)
+                    red[wv][s][(lane / TOP & 1) * NP + q.n0 + (lane / (TOP / 8) & 7)] = sum;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const int out = behind(t1 + i * NS, q.g, end);
+                const float b_ = from_groups<NS>(gb), a_ = from_groups<NS>(ga);
+                dD = fmaf(dys[i], x[i], dD);
+                const float dd = out ? 0.f : fmaf(LN2, a_, b_ * x[i]) * sd[i];
                 dbias += dd;
-                row_store(fmaf(dys[s], D, gb * dt[s]), dxp + t * yst, in ? q.nt : 0, q.vt);
-                row_store(dd, ddp + t * yst, in ? q.nt : 0, q.vt);
-                put_maps(sum, t, in);
-                __builtin_amdgcn_sched_barrier(0);
+                row_store(fmaf(dys[i], D, b_ * dt[i]), dxp + (t1 + i * NS) * yst, ROW_MAX, yoff | out);
+                row_store(dd, ddp + (t1 + i * NS) * yst, ROW_MAX, yoff | out);
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < K * 2 * NP; e += nthr) {
+                const int s = e / (2 * NP), i = e % (2 * NP);
+                float v = 0.f;
+                for (int w = 0; w < a.wpb; ++w) v += red[w][s][i];
+                if (t1 + s < end) put_map<T, NP>(a, v, om, pm, (t1 + s) * mst, i);
             }
         }
-        if (a.dh_in != nullptr)
-#pragma unroll
-            for (int n = 0; n < NP; ++n)
-                if (n < N) row_store(dh[n], a.dh_in + ((int64_t)row * N + n) * C + q.first, q.nf, q.vf);
+        if (a.dh_in != nullptr && ch == 0) store_state(a, q, a.dh_in + (int64_t)row * N * C, dh);
     }
-    float* part = a.part + ((int64_t)(p * a.slots + slot) * (N + 2)) * C + q.first;
+    float* part = a.part + ((int64_t)(p * a.slots + slot) * (N + 2)) * C;
+    store_state(a, q, part, dA);
+    float r[NS];
+    to_groups<NS>(dD, r);
+    dD = r[0];
 #pragma unroll
-    for (int n = 0; n < NP; ++n)
-        if (n < N) row_store(dA[n], part + (int64_t)n * C, q.nf, q.vf);
-    row_store(dD, part + (int64_t)N * C, q.nf, q.vf);
-    row_store(dbias, part + (int64_t)(N + 1) * C, q.nf, q.vf);
+    for (int j = 1; j < NS; ++j) dD += r[j];
+    to_groups<NS>(dbias, r);
+    dbias = r[0];
+#pragma unroll
+    for (int j = 1; j < NS; ++j) dbias += r[j];
+    const int po = q.g == 0 ? co : OOB;
+    row_store(dD, part + (int64_t)N * C + q.first, ROW_MAX, po);
+    row_store(dbias, part + (int64_t)(N + 1) * C + q.first, ROW_MAX, po);
 }
 
-// dB / dC: the channel blocks' partial sums, in order
+// dB / dC: the workgroups' partial sums, in order
 template <class T>
 __global__ __launch_bounds__(256) void ssm_maps_sum_kernel(const float* __restrict__ pB, const float* __restrict__ pC, T* __restrict__ dB, T* __restrict__ dC,
                                                            int nblk, int64_t n) {
@@ -291,6 +586,7 @@ __global__ __launch_bounds__(256) void ssm_maps_sum_kernel(const float* __restri
     }
 }
 
+// ---- host -------------------------------------------------------------------------------------------------------------------------------
 int scan_validate(const marlhip_ssm_shape* s) {
     if (ssm_validate(s, "ssm_scan") != 0) return -1;
     MARL_REQUIRE(s->state >= 1 && s->state <= SSM_MAX_STATE, "ssm_scan: %d states a channel (1..%d supported)", s->state, SSM_MAX_STATE);
@@ -298,16 +594,56 @@ int scan_validate(const marlhip_ssm_shape* s) {
     return 0;
 }
 
-int scan_blocks(const marlhip_ssm_shape* s) { return (s->channels / s->groups + 63) / 64; }
+struct ScanPlan {
+    int NS, nblk, chunk, nchunk, nck, wpb, wgs, slots;
+};
 
-// rows of one agent that a wave takes one after the other (its sums over rows stay in registers)
-int scan_slots(const marlhip_ssm_shape* s) {
-    const int64_t waves = 4096 / ((int64_t)s->n_agents * s->groups * scan_blocks(s));
-    const int64_t k = waves < 1 ? 1 : waves;
-    return (int)(s->batch < k ? s->batch : k);
+// How a call is split.  One wave a SIMD (1024 of them) is where the chip begins to be filled; a sequence of fewer is worth cutting into chunks,
+// which costs a first pass over delta, x and B (or dy, C) of about 0.8 of the second one: below half of that number only.
+ScanPlan scan_plan(const marlhip_ssm_shape* s) {
+    ScanPlan q;
+    q.NS = scan_np(s->state) / NL;
+    const int CL = 64 / q.NS;
+    q.nblk = (s->channels / s->groups + CL - 1) / CL;
+    q.nck = (s->steps + K - 1) / K;
+    const int64_t waves = (int64_t)s->n_agents * s->batch * s->groups * q.nblk;
+    q.nchunk = 1;
+    q.chunk = q.nck > 0 ? q.nck * K : K;
+    if (waves > 0 && waves <= 512 && s->steps >= 128) {
+        int64_t want = 2048 / waves, most = s->steps / 64;
+        if (want > most) want = most;
+        if (want > 1) {
+            q.chunk = (int)((q.nck + want - 1) / want) * K;
+            q.nchunk = (s->steps + q.chunk - 1) / q.chunk;
+        }
+    }
+    q.wpb = q.nblk < WMAX ? q.nblk : WMAX;
+    q.wgs = (q.nblk + q.wpb - 1) / q.wpb;
+    // items of one agent that a backward workgroup takes one after the other (its sums over them stay in registers)
+    const int64_t items = (int64_t)s->batch * q.nchunk, k = 4096 / ((int64_t)s->n_agents * s->groups * q.wgs * q.wpb);
+    q.slots = (int)(items < 1 ? 1 : (items < k ? items : (k < 1 ? 1 : k)));
+    return q;
 }
 
-ScanArgs scan_args(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q) {
+int64_t scan_items(const marlhip_ssm_shape* s, const ScanPlan& pl) { return (int64_t)s->n_agents * s->batch * pl.nchunk * s->groups * pl.nblk; }
+
+int seq_check(const char* what, const char* name, const marlhip_ssm_seq& q, int esize, int64_t steps) {
+    // a wave addresses up to 4 steps with 32-bit offsets
+    MARL_REQUIRE(q.data == nullptr || steps <= 1 || (q.step_stride >= 0 && q.step_stride * esize <= (1ll << 29)),
+                 "%s: %s has %lld elements between steps (0..2^29 bytes supported)", what, name, (long long)q.step_stride);
+    return 0;
+}
+int scan_seqs(const char* what, const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q, bool grad) {
+    const int e = s->dtype == 0 ? 4 : 2;
+    if (seq_check(what, "x", q->x, e, s->steps) || seq_check(what, "delta", q->delta, e, s->steps) || seq_check(what, "z", q->z, e, s->steps)) return -1;
+    if (grad && seq_check(what, "dy", q->dy, e, s->steps)) return -1;
+    MARL_REQUIRE(scan_items(s, scan_plan(s)) < (1ll << 31) - 8, "%s: batch %d x channels %d is too large", what, s->batch, s->channels);
+    MARL_REQUIRE(s->steps <= 1 || (int64_t)s->batch * s->channels * e <= (1ll << 29), "%s: batch %d x channels %d: a step is over 2^29 bytes", what, s->batch,
+                 s->channels);
+    return 0;
+}
+
+ScanArgs scan_args(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q, const ScanPlan& pl) {
     ScanArgs a = {};
     a.d = ssm_dims(s);
     a.x = ssm_seq(q->x); a.delta = ssm_seq(q->delta); a.Bm = ssm_seq(q->B); a.Cm = ssm_seq(q->C); a.z = ssm_seq(q->z); a.dy = ssm_seq(q->dy);
@@ -316,31 +652,55 @@ ScanArgs scan_args(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q) {
     a.y = q->y; a.dx = q->dx; a.ddelta = q->ddelta; a.dB = q->dB; a.dC = q->dC; a.dz = q->dz;
     a.h_out = q->h_out; a.record = q->record; a.dh_in = q->dh_in;
     a.softplus = q->softplus != 0;
-    a.nblk = scan_blocks(s);
-    const int K = scan_k_of(s->state);
-    a.nck = (s->steps + K - 1) / K;
+    a.nblk = pl.nblk; a.nck = pl.nck; a.chunk = pl.chunk; a.nchunk = pl.nchunk; a.wpb = pl.wpb; a.wgs = pl.wgs; a.slots = pl.slots;
     return a;
 }
 
-#define SSM_FOR_TYPE_AND_STATE(call)                                             \
-    do {                                                                         \
-        const int np_ = scan_np(s->state);                                       \
-        if (s->dtype == 0) { if (np_ == 8) { call(float, 8); } else if (np_ == 16) { call(float, 16); } else { call(float, 32); } }            \
-        else if (s->dtype == 1) { if (np_ == 8) { call(__bf16, 8); } else if (np_ == 16) { call(__bf16, 16); } else { call(__bf16, 32); } }    \
-        else { if (np_ == 8) { call(_Float16, 8); } else if (np_ == 16) { call(_Float16, 16); } else { call(_Float16, 32); } }                 \
-    } while (0)
+int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// f(type, lanes a channel)
+template <class F>
+void by_type_and_state(const marlhip_ssm_shape* s, int NS, F f) {
+    auto by_ns = [&](auto t) {
+        if (NS == 1) f(t, Idx<1>{});
+        else if (NS == 2) f(t, Idx<2>{});
+        else f(t, Idx<4>{});
+    };
+    if (s->dtype == 0) by_ns(float{});
+    else if (s->dtype == 1) by_ns(__bf16{});
+    else by_ns(_Float16{});
+}
+
+struct CarryWs {
+    int64_t carry, sums, total;
+};
+CarryWs carry_ws(const marlhip_ssm_shape* s, const ScanPlan& pl) {
+    CarryWs w = {0, 0, 0};
+    if (pl.nchunk <= 1) return w;
+    const int64_t rows = (int64_t)s->n_agents * s->batch * pl.nchunk;
+    w.sums = round256(rows * s->state * s->channels * 4);
+    w.total = w.sums + round256(rows * s->channels * 4);
+    return w;
+}
+
+int join(const ScanArgs& a, const float* start, int reverse, hipStream_t st) {
+    const int64_t wgs = (int64_t)a.d.P * a.d.B * a.d.N * ((a.d.C + 63) / 64);
+    MARL_REQUIRE(wgs < (1ll << 31), "ssm_scan: too many rows");
+    hipLaunchKernelGGL(ssm_scan_join_kernel, dim3((unsigned)wgs), dim3(1024), 0, st, a, start, reverse);
+    MARL_CHECK_LAUNCH("ssm_scan_join_kernel");
+    return 0;
+}
 
 }  // namespace
 
 extern "C" int64_t marlhip_ssm_scan_record_floats(const marlhip_ssm_shape* s) {
     if (scan_validate(s) != 0) return -1;
-    const int K = scan_k_of(s->state);
     return (int64_t)s->n_agents * s->batch * ((s->steps + K - 1) / K) * s->state * s->channels;
 }
 
 extern "C" int64_t marlhip_ssm_scan_workspace_bytes(const marlhip_ssm_shape* s) {
     if (scan_validate(s) != 0) return -1;
-    return 0;
+    return carry_ws(s, scan_plan(s)).total;
 }
 
 extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -348,16 +708,28 @@ extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_sc
     MARL_REQUIRE(q != nullptr && q->A != nullptr, "ssm_scan: NULL argument");
     const bool any = s->steps > 0 && s->batch > 0;
     MARL_REQUIRE(!any || (q->x.data && q->delta.data && q->B.data && q->C.data && q->y), "ssm_scan: NULL pointer");
-    const int64_t need = marlhip_ssm_scan_workspace_bytes(s);
-    MARL_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "ssm_scan: workspace of %lld bytes needed, %lld given", (long long)need,
+    if (scan_seqs("ssm_scan", s, q, false) != 0) return -1;
+    const ScanPlan pl = scan_plan(s);
+    const CarryWs w = carry_ws(s, pl);
+    MARL_REQUIRE(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total), "ssm_scan: workspace of %lld bytes needed, %lld given", (long long)w.total,
                  (long long)workspace_bytes);
     if (s->batch == 0) return 0;
-    ScanArgs a = scan_args(s, q);
-    a.items = (int64_t)s->n_agents * s->batch * s->groups * a.nblk;
-    MARL_REQUIRE((a.items + 3) / 4 < (1ll << 31), "ssm_scan: too many rows");
-#define SCAN_FWD(T, NP) hipLaunchKernelGGL((ssm_scan_fwd_kernel<T, NP>), dim3((unsigned)((a.items + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a)
-    SSM_FOR_TYPE_AND_STATE(SCAN_FWD);
-#undef SCAN_FWD
+    ScanArgs a = scan_args(s, q, pl);
+    a.items = (int)scan_items(s, pl);
+    const dim3 grid((unsigned)((a.items + 3) / 4));
+    hipStream_t st = (hipStream_t)stream;
+    if (pl.nchunk > 1) {
+        a.carry = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.carry);
+        a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.sums);
+        by_type_and_state(s, pl.NS, [&](auto t, auto ns) {
+            hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(ns)::v, true>), grid, dim3(256), 0, st, a);
+        });
+        MARL_CHECK_LAUNCH("ssm_scan_fwd_kernel");
+        if (join(a, a.h_in, 0, st) != 0) return -2;
+    }
+    by_type_and_state(s, pl.NS, [&](auto t, auto ns) {
+        hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(ns)::v, false>), grid, dim3(256), 0, st, a);
+    });
     MARL_CHECK_LAUNCH("ssm_scan_fwd_kernel");
     return 0;
 }
@@ -365,17 +737,17 @@ extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_sc
 namespace {
 struct GradWs {
     int64_t pB, pC, part, total;
-    int slots;
+    CarryWs carry;
 };
-GradWs grad_ws(const marlhip_ssm_shape* s) {
+GradWs grad_ws(const marlhip_ssm_shape* s, const ScanPlan& pl) {
     GradWs w;
-    int64_t off = 0;
-    auto take = [&](int64_t floats) { const int64_t o = off; off += (floats * 4 + 255) / 256 * 256; return o; };
-    const int64_t maps = scan_blocks(s) > 1 ? (int64_t)scan_blocks(s) * s->n_agents * s->steps * s->batch * s->groups * s->state : 0;
+    w.carry = carry_ws(s, pl);
+    int64_t off = w.carry.total;
+    auto take = [&](int64_t floats) { const int64_t o = off; off += round256(floats * 4); return o; };
+    const int64_t maps = pl.wgs > 1 ? (int64_t)pl.wgs * s->n_agents * s->steps * s->batch * s->groups * s->state : 0;
     w.pB = take(maps);
     w.pC = take(maps);
-    w.slots = scan_slots(s);
-    w.part = take((int64_t)s->n_agents * w.slots * (s->state + 2) * s->channels);
+    w.part = take((int64_t)s->n_agents * pl.slots * (s->state + 2) * s->channels);
     w.total = off;
     return w;
 }
@@ -383,7 +755,7 @@ GradWs grad_ws(const marlhip_ssm_shape* s) {
 
 extern "C" int64_t marlhip_ssm_scan_grad_workspace_bytes(const marlhip_ssm_shape* s) {
     if (scan_validate(s) != 0) return -1;
-    return grad_ws(s).total;
+    return grad_ws(s, scan_plan(s)).total;
 }
 
 extern "C" int marlhip_ssm_scan_grad(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -393,37 +765,45 @@ extern "C" int marlhip_ssm_scan_grad(const marlhip_ssm_shape* s, const marlhip_s
     MARL_REQUIRE(!any || (q->x.data && q->delta.data && q->B.data && q->C.data && q->dy.data && q->record && q->dx && q->ddelta && q->dB && q->dC),
                  "ssm_scan_grad: NULL pointer");
     MARL_REQUIRE(!any || (q->z.data == nullptr) == (q->dz == nullptr), "ssm_scan_grad: dz goes with z");
-    const GradWs w = grad_ws(s);
-    MARL_REQUIRE(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total), "ssm_scan_grad: workspace of %lld bytes needed, %lld given",
-                 (long long)w.total, (long long)workspace_bytes);
-    ScanArgs a = scan_args(s, q);
+    if (scan_seqs("ssm_scan_grad", s, q, true) != 0) return -1;
+    const ScanPlan pl = scan_plan(s);
+    const GradWs w = grad_ws(s, pl);
+    MARL_REQUIRE(workspace != nullptr && workspace_bytes >= w.total, "ssm_scan_grad: workspace of %lld bytes needed, %lld given", (long long)w.total,
+                 (long long)workspace_bytes);
+    ScanArgs a = scan_args(s, q, pl);
     char* ws = static_cast<char*>(workspace);
-    const int64_t maps = (int64_t)s->n_agents * s->steps * s->batch * s->groups * s->state;
-    a.slots = w.slots;
+    hipStream_t st = (hipStream_t)stream;
     a.part = reinterpret_cast<float*>(ws + w.part);
-    if (a.nblk > 1) {
+    if (pl.wgs > 1) {
         a.pB = reinterpret_cast<float*>(ws + w.pB);
         a.pC = reinterpret_cast<float*>(ws + w.pC);
     }
-    a.items = (int64_t)s->n_agents * w.slots * s->groups * a.nblk;
-    hipStream_t st = (hipStream_t)stream;
-    if (a.items > 0) {
-#define SCAN_BWD(T, NP) hipLaunchKernelGGL((ssm_scan_bwd_kernel<T, NP>), dim3((unsigned)((a.items + 3) / 4)), dim3(256), 0, st, a)
-        SSM_FOR_TYPE_AND_STATE(SCAN_BWD);
-#undef SCAN_BWD
-        MARL_CHECK_LAUNCH("ssm_scan_bwd_kernel");
-        if (a.nblk > 1 && maps > 0) {
-            const unsigned blocks = (unsigned)((maps + 255) / 256 < 4096 ? (maps + 255) / 256 : 4096);
-#define MAPS_SUM(T) hipLaunchKernelGGL((ssm_maps_sum_kernel<T>), dim3(blocks), dim3(256), 0, st, a.pB, a.pC, (T*)q->dB, (T*)q->dC, a.nblk, maps)
-            if (s->dtype == 0) MAPS_SUM(float);
-            else if (s->dtype == 1) MAPS_SUM(__bf16);
-            else MAPS_SUM(_Float16);
+    if (pl.nchunk > 1) {
+        a.carry = reinterpret_cast<float*>(ws + w.carry.carry);
+        a.sums = reinterpret_cast<float*>(ws + w.carry.sums);
+        a.items = (int)scan_items(s, pl);
+        const dim3 grid((unsigned)((a.items + 3) / 4));
+        by_type_and_state(s, pl.NS, [&](auto t, auto ns) {
+            hipLaunchKernelGGL((ssm_scan_bwd_carry_kernel<decltype(t), decltype(ns)::v>), grid, dim3(256), 0, st, a);
+        });
+        MARL_CHECK_LAUNCH("ssm_scan_bwd_carry_kernel");
+        if (join(a, a.dh_out, 1, st) != 0) return -2;
+    }
+    const dim3 grid((unsigned)(s->n_agents * pl.slots * s->groups * pl.wgs)), block(64 * pl.wpb);
+    by_type_and_state(s, pl.NS, [&](auto t, auto ns) { hipLaunchKernelGGL((ssm_scan_bwd_kernel<decltype(t), decltype(ns)::v>), grid, block, 0, st, a); });
+    MARL_CHECK_LAUNCH("ssm_scan_bwd_kernel");
+    const int64_t maps = (int64_t)s->n_agents * s->steps * s->batch * s->groups * s->state;
+    if (pl.wgs > 1 && maps > 0) {
+        const unsigned blocks = (unsigned)((maps + 255) / 256 < 4096 ? (maps + 255) / 256 : 4096);
+#define MAPS_SUM(T) hipLaunchKernelGGL((ssm_maps_sum_kernel<T>), dim3(blocks), dim3(256), 0, st, a.pB, a.pC, (T*)q->dB, (T*)q->dC, pl.wgs, maps)
+        if (s->dtype == 0) MAPS_SUM(float);
+        else if (s->dtype == 1) MAPS_SUM(__bf16);
+        else MAPS_SUM(_Float16);
 #undef MAPS_SUM
-            MARL_CHECK_LAUNCH("ssm_maps_sum_kernel");
-        }
+        MARL_CHECK_LAUNCH("ssm_maps_sum_kernel");
     }
     const int64_t cols = (int64_t)(s->state + 2) * s->channels;
-    hipLaunchKernelGGL(ssm_weights_sum_kernel, dim3((unsigned)((cols + 63) / 64), a.d.M), dim3(256), 0, st, a.d, w.slots, s->state, 2, a.part, q->dA, q->dD,
+    hipLaunchKernelGGL(ssm_weights_sum_kernel, dim3((unsigned)((cols + 63) / 64), a.d.M), dim3(256), 0, st, a.d, pl.slots, s->state, 2, a.part, q->dA, q->dD,
                        q->ddelta_bias);
     MARL_CHECK_LAUNCH("ssm_weights_sum_kernel");
     return 0;

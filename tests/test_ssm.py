@@ -309,11 +309,11 @@ def test_scan_expanded_inputs_and_odd_strides():
 
 @pytest.mark.gpu
 def test_scan_offsets_beyond_32_bits():
-    """steps 2^30 elements apart: the last one starts 6 GiB into the buffer"""
-    P, S, B, C, N = 1, 4, 2, 66, 5
+    """steps 2^28 elements (2^29 bytes) apart: the last one starts 5.5 GiB into the buffer"""
+    P, S, B, C, N = 1, 12, 2, 66, 10
     v = make_scan(P, S, B, C, N, dtype=BF16)
-    big = torch.empty(3 * 2**30 + B * C, dtype=BF16, device="cuda")
-    x = big.as_strided((P, S, B, C), (0, 2**30, C, 1))
+    big = torch.empty(11 * 2**28 + B * C, dtype=BF16, device="cuda")
+    x = big.as_strided((P, S, B, C), (0, 2**28, C, 1))
     x.copy_(v["x"])
     v["x"] = x
     check_scan(v)
@@ -741,6 +741,19 @@ def test_scan_refuses(name, spoil, text):
         scan_grad_call(v, rec)
 
 
+def far_apart():
+    """a scan over steps more than 2^29 bytes apart (pointers that nothing reads: the call is refused)"""
+    import ctypes
+
+    from codebase_amd._lib import SsmScanArgs, SsmSeq, SsmShape
+
+    a = SsmScanArgs()
+    a.x = a.delta = a.B = a.C = SsmSeq(256, 0, 16, 16)
+    a.delta = SsmSeq(256, 0, 2**27 + 1, 16)
+    a.A, a.y = 256, 256
+    return ctypes.byref(SsmShape(1, 2, 3, 12, 4, 1, 0, 0)), ctypes.byref(a), None, 0, None
+
+
 def test_scan_refuses_sizes_and_states():
     v = make_scan(2, 5, 3, 12, 4, G=2, device="cpu")
     with pytest.raises(ValueError, match="record is missing"):
@@ -756,6 +769,8 @@ def test_scan_refuses_sizes_and_states():
         scan_grad_call(dict(v, dy=v["dy"][:, 1:]), h.ssm_scan_record(v["x"], 4))
     with pytest.raises(ValueError, match="dh_out has shape"):
         scan_grad_call(dict(v, dh_out=v["dh_out"][..., 1:]), h.ssm_scan_record(v["x"], 4))
+    with pytest.raises(h.MarlHipError, match="2\\^29 bytes"):
+        h.check(h.lib.marlhip_ssm_scan(*far_apart()))
     with pytest.raises(h.MarlHipError, match="33 states"):
         h.ssm_scan_record(v["x"], 33)
     with pytest.raises(h.MarlHipError, match="17 agents"):
