@@ -136,40 +136,55 @@ __device__ __forceinline__ float half_sum(float lo, float hi, int lane) {
     }
 }
 
-// Sums of 8 pairs over the TOP * 2 lanes of a group, formed as the pairs appear: f(n, b, c) gives (b_n, c_n).  The pairs merge as soon as two
+// Sums of NL pairs over the TOP * 2 lanes of a group, formed as the pairs appear: f(n, b, c) gives (b_n, c_n).  The pairs merge as soon as two
 // exist - about 2 instructions a value, where a butterfly each would take 2 log2(lanes) - and need a handful of registers.  gfx950's lane
 // swaps exchange halves of two registers in one instruction; inside a row of 16 lanes the partners are mirrors (DPP).  Lane bit TOP tells b
-// from c, the three below it are n; lanes that differ in lower bits only hold shares of the same sum (TOP 32: xor 2 and 1, TOP 16: xor 1).
-template <int TOP, int LVL, int I, class F>
+// from c, the log2(NL) below it are n; lanes that differ in lower bits only hold the same sum.
+template <int NL, int TOP, int LVL, int I, class F>
 __device__ __forceinline__ float pair_tree(F& f, int lane) {
     if constexpr (LVL == 0) {
         float b, c;
         f(Idx<I>{}, b, c);
         return half_sum<TOP>(b, c, lane);
     } else {
-        const float lo = pair_tree<TOP, LVL - 1, I>(f, lane), hi = pair_tree<TOP, LVL - 1, I + (8 >> LVL)>(f, lane);
+        const float lo = pair_tree<NL, TOP, LVL - 1, I>(f, lane), hi = pair_tree<NL, TOP, LVL - 1, I + (NL >> LVL)>(f, lane);
         return half_sum<(TOP >> LVL)>(lo, hi, lane);
     }
+}
+template <int NL, int TOP, class F>
+__device__ __forceinline__ float pair_sums(F& f, int lane) {
+    static_assert(NL == 4 || NL == 8, "4 or 8 pairs");
+    float v = pair_tree<NL, TOP, NL == 8 ? 3 : 2, 0>(f, lane);
+    if constexpr (TOP / NL > 4) v += dpp_half_mirror(v);
+    if constexpr (TOP / NL > 2) v += dpp_xor3(v);
+    if constexpr (TOP / NL > 1) v += dpp_xor1(v);
+    return v;
 }
 
 // The gradients of one network's weights: the partial sums [agent][slot][rows + extra][C] of its agents, in order.  The first `rows` rows go
 // to d0, the next to d1, the one after that to d2 (NULL: not wanted).
-static __global__ __launch_bounds__(256) void ssm_weights_sum_kernel(SsmDims d, int slots, int rows, int extra, const float* __restrict__ part,
-                                                                     float* __restrict__ d0, float* __restrict__ d1, float* __restrict__ d2) {
+// A workgroup takes 64 columns, its 16 waves every 16th slot with eight requests in flight each (bound by latency: the sums are small).
+static __global__ __launch_bounds__(1024) void ssm_weights_sum_kernel(SsmDims d, int slots, int rows, int extra, const float* __restrict__ part,
+                                                                      float* __restrict__ d0, float* __restrict__ d1, float* __restrict__ d2) {
     const int m = blockIdx.y;
     const int64_t n = (int64_t)(rows + extra) * d.C;
-    __shared__ float red[4][64];
+    __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
     const int64_t i = (int64_t)blockIdx.x * 64 + lane;
     float s = 0.f;
     if (i < n)
         for (int p = 0; p < d.P; ++p)
-            if (d.net[p] == m)
-                for (int k = q; k < slots; k += 4) s += part[((int64_t)p * slots + k) * n + i];
+            if (d.net[p] == m) {
+                const float* src = part + (int64_t)p * slots * n + i;
+#pragma unroll 8
+                for (int k = q; k < slots; k += 16) s += src[k * n];
+            }
     red[q][lane] = s;
     __syncthreads();
     if (q != 0 || i >= n) return;
-    s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][lane];
     const int64_t r = i / d.C, c = i % d.C;
     if (r < rows) d0[((int64_t)m * rows + r) * d.C + c] = s;
     else if (r == rows) { if (d1 != nullptr) d1[(int64_t)m * d.C + c] = s; }

@@ -371,7 +371,7 @@ extern "C" int marlhip_ssm_conv_grad(const marlhip_ssm_shape* s, const marlhip_s
     a.part = static_cast<float*>(workspace);
     if (conv_bwd_any(s, a, (hipStream_t)stream) != 0) return -1;
     const int64_t cols = (int64_t)(a.W + 1) * a.d.C;
-    hipLaunchKernelGGL(ssm_weights_sum_kernel, dim3((unsigned)((cols + 63) / 64), a.d.M), dim3(256), 0, (hipStream_t)stream, a.d, a.slots, a.W, 1, a.part,
+    hipLaunchKernelGGL(ssm_weights_sum_kernel, dim3((unsigned)((cols + 63) / 64), a.d.M), dim3(1024), 0, (hipStream_t)stream, a.d, a.slots, a.W, 1, a.part,
                        q->dweight, q->dbias, (float*)nullptr);
     MARL_CHECK_LAUNCH("ssm_weights_sum_kernel");
     return 0;

@@ -8,13 +8,13 @@
 // shares of y.  So NS > 1 costs three swaps a step, keeps 8 / N of the registers and gives NS times the waves, which is what small batches need.
 // B and C of a step are the same for a group's channels and come as LDS broadcasts, K steps at a time.
 #include "ssm.h"
+#include <stdlib.h>
 
 using namespace marl;
 
 namespace {
 
 constexpr int K = 8;     // steps of a block: between two recorded states
-constexpr int NL = 8;    // states a lane keeps
 constexpr int WMAX = 8;  // waves of a backward workgroup
 
 struct ScanArgs {
@@ -33,10 +33,8 @@ struct ScanArgs {
     int items;
 };
 
-inline int scan_np(int N) { return N <= 8 ? 8 : (N <= 16 ? 16 : 32); }
-
 // ---- a wave's place ------------------------------------------------------------------------------------------------------------------
-template <class T, int NS>
+template <int NL, int NS>
 struct Lane {
     static constexpr int CL = 64 / NS;
     int lane, g, cl;      // group, channel within the block
@@ -54,22 +52,25 @@ struct Lane {
         act = first + cl < (grp + 1) * Cg;
         n0 = g * NL;
     }
-    // offset of this lane's element of state n in an [N][C] array from its first channel
-    __device__ __forceinline__ int state_off(const ScanArgs& a, int n) const { return act && n0 + n < a.d.N ? ((n0 + n) * a.d.C + cl) * 4 : OOB; }
+    // this lane's element of an [N][C] array: its offset from state n of the first channel, for every n; states from N on are not there
+    __device__ __forceinline__ int state_off(const ScanArgs& a) const { return act ? (n0 * a.d.C + cl) * 4 : OOB; }
+    __device__ __forceinline__ int no_state(const ScanArgs& a, int n) const { return (a.d.N - 1 - n - n0) & OOB; }
     __device__ __forceinline__ int chan_off(int bytes) const { return act ? cl * bytes : OOB; }
 };
 
-template <class T, int NS>
-__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<T, NS>& q, const float* p, float scale, float (&r)[NL]) {
+template <int NL, int NS>
+__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<NL, NS>& q, const float* p, float scale, float (&r)[NL]) {
+    const int off = q.state_off(a), bytes = p != nullptr ? ROW_MAX : 0;
 #pragma unroll
-    for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first, p != nullptr ? ROW_MAX : 0, q.state_off(a, n));
+    for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first + (int64_t)n * a.d.C, bytes, off | q.no_state(a, n));
 #pragma unroll
     for (int n = 0; n < NL; ++n) r[n] *= scale;
 }
-template <class T, int NS>
-__device__ __forceinline__ void store_state(const ScanArgs& a, const Lane<T, NS>& q, float* p, const float (&r)[NL]) {
+template <int NL, int NS>
+__device__ __forceinline__ void store_state(const ScanArgs& a, const Lane<NL, NS>& q, float* p, const float (&r)[NL]) {
+    const int off = q.state_off(a);
 #pragma unroll
-    for (int n = 0; n < NL; ++n) row_store(r[n], p + q.first, ROW_MAX, q.state_off(a, n));
+    for (int n = 0; n < NL; ++n) row_store(r[n], p + q.first + (int64_t)n * a.d.C, ROW_MAX, off | q.no_state(a, n));
 }
 
 // value of group i of a register that holds one value a group, in every group
@@ -115,17 +116,20 @@ struct Raw {
     __device__ __forceinline__ void load(const T* p, int voff) { v = __builtin_amdgcn_raw_buffer_load_b16(row_rsrc(p, ROW_MAX), voff, 0, 0); }
 };
 
-// offset of step t0 + i NS + g of a sequence from step t0 + i NS; steps from `end` on are not there
+// A sequence's steps for a wave: a uniform pointer to step t (moved by adding, no product a load) and this lane's offset to its own step t + g
 template <class T, int NS>
 struct SeqPtr {
-    const T* p;
-    int64_t st;
+    const char* p;
+    int64_t st;  // bytes between steps
     int voff;
-    __device__ __forceinline__ SeqPtr(const SsmSeq& s, const Lane<T, NS>& q, int pa, int b)
-        : p(seq_at<T>(s, pa, b) + q.first), st(s.st), voff(q.act ? q.g * (int)(s.st * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB) {}
-    __device__ __forceinline__ void load(Raw<T>& r, int64_t t, int out) const { r.load(p + t * st, voff | out); }
+    template <int NL>
+    __device__ __forceinline__ SeqPtr(const SsmSeq& s, const Lane<NL, NS>& q, int pa, int b, int t)
+        : p(reinterpret_cast<const char*>(seq_at<T>(s, pa, b) + q.first + t * s.st)), st(s.st * (int64_t)sizeof(T)),
+          voff(q.act ? q.g * (int)(s.st * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB) {}
+    __device__ __forceinline__ void load(Raw<T>& r, int steps, int out) const { r.load(reinterpret_cast<const T*>(p + steps * st), voff | out); }
+    __device__ __forceinline__ void move(int steps) { p += steps * st; }
 };
-// -1's sign bit where step t + g is behind the end: OR-ed into an offset it points behind any row
+// the sign bit where step t + g is behind the end: OR-ed into an offset it points behind any row
 __device__ __forceinline__ int behind(int t, int g, int end) { return (end - 1 - t - g) & OOB; }
 
 // B / C of K steps: what this thread of NT carries to LDS
@@ -133,28 +137,48 @@ template <class T, int NP, int NT>
 struct Maps {
     static constexpr int M = (K * NP + NT - 1) / NT;
     Raw<T> b[M], c[M];
-    __device__ __forceinline__ void load(const ScanArgs& a, const T* Bp, const T* Cp, int t0, int end, int tid) {
+};
+template <class T, int NP, int NT>
+struct MapsPtr {
+    static constexpr int M = (K * NP + NT - 1) / NT;
+    const char *pb, *pc;  // step t
+    int64_t sb, sc;
+    int vb[M], vc[M];
+    __device__ __forceinline__ MapsPtr(const ScanArgs& a, int pa, int b, int grp, int t, int tid)
+        : pb(reinterpret_cast<const char*>(seq_at<T>(a.Bm, pa, b) + grp * a.d.N + t * a.Bm.st)),
+          pc(reinterpret_cast<const char*>(seq_at<T>(a.Cm, pa, b) + grp * a.d.N + t * a.Cm.st)), sb(a.Bm.st * (int64_t)sizeof(T)), sc(a.Cm.st * (int64_t)sizeof(T)) {
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             const int e = tid + NT * i, s = e / NP, n = e % NP;
-            const bool ok = e < K * NP && n < a.d.N && t0 + s < end;
-            const int64_t t = ok ? t0 + s : t0, m = ok ? n : 0;
-            b[i].v = reinterpret_cast<const decltype(b[i].v)*>(Bp)[t * a.Bm.st + m];
-            c[i].v = reinterpret_cast<const decltype(c[i].v)*>(Cp)[t * a.Cm.st + m];
-            if (!ok) b[i].v = 0, c[i].v = 0;
+            const bool ok = e < K * NP && n < a.d.N;
+            vb[i] = ok ? s * (int)sb + n * (int)sizeof(T) : OOB;
+            vc[i] = ok ? s * (int)sc + n * (int)sizeof(T) : OOB;
         }
     }
-    __device__ __forceinline__ void store(float* lb, float* lc, int tid) const {
+    __device__ __forceinline__ void load(Maps<T, NP, NT>& m, int t, int end, int tid) const {  // t: where the pointers are
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-            const int e = tid + NT * i;
-            if (NT * M == K * NP || e < K * NP) {
-                lb[e] = b[i].get();
-                lc[e] = c[i].get();
-            }
+            const int out = behind(t, (tid + NT * i) / NP, end);
+            m.b[i].load(reinterpret_cast<const T*>(pb), vb[i] | out);
+            m.c[i].load(reinterpret_cast<const T*>(pc), vc[i] | out);
         }
     }
+    __device__ __forceinline__ void move(int steps) {
+        pb += steps * sb;
+        pc += steps * sc;
+    }
 };
+template <class T, int NP, int NT>
+__device__ __forceinline__ void store_maps(const Maps<T, NP, NT>& m, float* lb, float* lc, int tid) {
+#pragma unroll
+    for (int i = 0; i < Maps<T, NP, NT>::M; ++i) {
+        const int e = tid + NT * i;
+        if (NT * Maps<T, NP, NT>::M == K * NP || e < K * NP) {
+            lb[e] = m.b[i].get();
+            lc[e] = m.c[i].get();
+        }
+    }
+}
 
 // bit s: an episode starts at step t0 + s
 __device__ __forceinline__ int load_reset(const ScanArgs& a, int b, int t0, int end, int lane) {
@@ -164,6 +188,14 @@ __device__ __forceinline__ int load_reset(const ScanArgs& a, int b, int t0, int 
 }
 __device__ __forceinline__ unsigned reset_bits(int v) { return (unsigned)__builtin_amdgcn_ballot_w64(v != 0) & ((1u << K) - 1); }
 
+// Resets are rare and the same for a whole wave: a branch, which the empty asm keeps the compiler from turning into a select a state
+template <int NL>
+__device__ __forceinline__ void clear(float (&h)[NL]) {
+    asm volatile("");
+#pragma unroll
+    for (int n = 0; n < NL; ++n) h[n] = 0.f;
+}
+
 __device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bias) {
     const float r = d + bias;
     return a.softplus ? softplus(r) : r;
@@ -171,7 +203,7 @@ __device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bia
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
 // CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass)
-template <class T, int NS, bool CARRY>
+template <class T, int NL, int NS, bool CARRY>
 __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     constexpr int NP = NS * NL, KG = K / NS;
     __shared__ float lds[4][2][K * NP];
@@ -180,27 +212,31 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     if (item >= a.items) return;
     const int ncb = a.d.G * a.nblk, rc = uni(item / ncb), cb = item - rc * ncb;  // rc: (row, chunk)
     const int row = uni(rc / a.nchunk), ch = rc - row * a.nchunk, p = uni(row / a.d.B), b = row - p * a.d.B;
-    const Lane<T, NS> q(a, cb, threadIdx.x & 63);
+    const Lane<NL, NS> q(a, cb, threadIdx.x & 63);
     const int N = a.d.N, C = a.d.C, net = a.d.net[p], len = uni(seq_len(a.lengths, b, a.d.S));
     const int first = ch * a.chunk, last = first + a.chunk < a.d.S ? first + a.chunk : a.d.S, end = len < last ? len : last;
-    const SeqPtr<T, NS> xs(a.x, q, p, b), ds(a.delta, q, p, b), zs(a.z, q, p, b);
-    const T *Bp = seq_at<T>(a.Bm, p, b) + q.grp * N, *Cp = seq_at<T>(a.Cm, p, b) + q.grp * N;
+    SeqPtr<T, NS> xs(a.x, q, p, b, first), ds(a.delta, q, p, b, first), zs(a.z, q, p, b, first);
+    MapsPtr<T, NP, 64> ms(a, p, b, q.grp, first, threadIdx.x & 63);
     const bool gated = !CARRY && a.z.data != nullptr;
     const int lane = q.lane;
 
     Raw<T> x[KG], dr[KG], z[KG];
     Maps<T, NP, 64> maps;
     int rs;
-    auto request = [&](int t0) __attribute__((always_inline)) {
+    auto request = [&](int t0) __attribute__((always_inline)) {  // the pointers are at t0
 #pragma unroll
         for (int i = 0; i < KG; ++i) {
             const int out = behind(t0 + i * NS, q.g, end);
-            xs.load(x[i], t0 + i * NS, out);
-            ds.load(dr[i], t0 + i * NS, out);
-            if (gated) zs.load(z[i], t0 + i * NS, out);
+            xs.load(x[i], i * NS, out);
+            ds.load(dr[i], i * NS, out);
+            if (gated) zs.load(z[i], i * NS, out);
         }
-        maps.load(a, Bp, Cp, t0, end, lane);
+        ms.load(maps, t0, end, lane);
         rs = load_reset(a, b, t0, end, lane);
+        xs.move(K);
+        ds.move(K);
+        zs.move(K);
+        ms.move(K);
     };
     if (first < end) request(first);
     float A[NL], h[NL];
@@ -210,14 +246,14 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     const int co = q.chan_off(4);
     const float D = row_load(a.D + (int64_t)net * C + q.first, a.D != nullptr ? ROW_MAX : 0, co);
     const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, co);
-    T* yp = static_cast<T*>(a.y) + ((int64_t)p * a.d.S * a.d.B + b) * C + q.first;
     const int64_t yst = (int64_t)a.d.B * C;
+    T* yp = static_cast<T*>(a.y) + ((int64_t)p * a.d.S * a.d.B + b) * C + q.first + first * yst;  // at step t0
     const int yoff = q.act ? q.g * (int)(yst * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB;
     float *lb = lds[wv][0], *lc = lds[wv][1];
     float total = 0.f;  // CARRY: sum of dt
     for (int t0 = first; t0 < end; t0 += K) {
         wave_lds_sync();
-        maps.store(lb, lc, lane);
+        store_maps(maps, lb, lc, lane);
         const unsigned fresh = reset_bits(rs);
         float xv[KG], dt[KG], gate[KG];
 #pragma unroll
@@ -229,35 +265,44 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
         wave_lds_sync();
         if (t0 + K < end) request(t0 + K);
         if (!CARRY && a.record != nullptr) store_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, h);
+        // two forms of the same steps: a whole block without resets is straight-line code, so that the maps' LDS reads run ahead of their use;
+        // resets (a select a state) and ends inside a block go through the other one
+        auto steps = [&](auto plain) __attribute__((always_inline)) {
+            constexpr bool PLAIN = decltype(plain)::v;
 #pragma unroll
-        for (int i = 0; i < KG; ++i) {
-            if (t0 + i * NS >= end) break;
-            const int out = behind(t0 + i * NS, q.g, end);
-            const float dti = out ? 0.f : dt[i];
-            float dts[NS], us[NS], ys[NS];
-            to_groups<NS>(dti, dts);
-            to_groups<NS>(dti * xv[i], us);
-            if (CARRY) total += fresh >> (i * NS + q.g) & 1 ? __builtin_nanf("") : dti;
-#pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                const int s = i * NS + j;
-                if (fresh >> s & 1)
-#pragma unroll
-                    for (int n = 0; n < NL; ++n) h[n] = 0.f;
-                float y = 0.f;
-#pragma unroll
-                for (int n = 0; n < NL; ++n) {
-                    h[n] = fmaf(exp2_fast(dts[j] * A[n]), h[n], us[j] * lb[s * NP + q.n0 + n]);
-                    if (!CARRY) y = fmaf(h[n], lc[s * NP + q.n0 + n], y);
+            for (int i = 0; i < KG; ++i) {
+                int out = 0;
+                if (!PLAIN) {
+                    if (t0 + i * NS >= end) break;
+                    out = behind(t0 + i * NS, q.g, end);
+                    if (out) dt[i] = 0.f;
                 }
-                ys[j] = y;
+                float dts[NS], us[NS], ys[NS];
+                to_groups<NS>(dt[i], dts);
+                to_groups<NS>(dt[i] * xv[i], us);
+                if (CARRY) total += !PLAIN && (fresh >> (i * NS + q.g) & 1) ? __builtin_nanf("") : dt[i];
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    const int s = i * NS + j;
+                    const bool re = !PLAIN && (fresh >> s & 1);
+                    float y = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NL; ++n) {
+                        h[n] = fmaf(exp2_fast(dts[j] * A[n]), re ? 0.f : h[n], us[j] * lb[s * NP + q.n0 + n]);
+                        if (!CARRY) y = fmaf(h[n], lc[s * NP + q.n0 + n], y);
+                    }
+                    ys[j] = y;
+                }
+                if (!CARRY) {
+                    float y = fmaf(D, xv[i], from_groups<NS>(ys));
+                    if (gated) y *= gate[i] * sigmoid(gate[i]);
+                    row_store(y, yp + i * NS * yst, ROW_MAX, yoff | out);
+                }
             }
-            if (!CARRY) {
-                float y = fmaf(D, xv[i], from_groups<NS>(ys));
-                if (gated) y *= gate[i] * sigmoid(gate[i]);
-                row_store(y, yp + (t0 + i * NS) * yst, ROW_MAX, yoff | out);
-            }
-        }
+        };
+        if (t0 + K <= end && fresh == 0) steps(Idx<1>{});
+        else steps(Idx<0>{});
+        yp += K * yst;
     }
     if (CARRY) {
         store_state(a, q, a.carry + ((int64_t)row * a.nchunk + ch) * N * C, h);
@@ -269,6 +314,7 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
         row_store(total, a.sums + ((int64_t)row * a.nchunk + ch) * C + q.first, ROW_MAX, q.g == 0 ? co : OOB);
         return;
     }
+    yp = static_cast<T*>(a.y) + ((int64_t)p * a.d.S * a.d.B + b) * C + q.first;
     for (int t = end > first ? end : first; t < last; ++t) row_store(0.f, yp + t * yst, ROW_MAX, q.g == 0 ? q.chan_off(sizeof(T)) : OOB);
     if (a.h_out != nullptr && ch == a.nchunk - 1) store_state(a, q, a.h_out + (int64_t)row * N * C, h);
 }
@@ -307,10 +353,26 @@ __global__ __launch_bounds__(1024) void ssm_scan_join_kernel(ScanArgs a, const f
     }
 }
 
+// The same for few chunks: a thread takes a state of a channel through all of them.
+__global__ __launch_bounds__(256) void ssm_scan_join_few_kernel(ScanArgs a, const float* __restrict__ start, int reverse) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, nc = (int64_t)a.d.N * a.d.C;
+    if (i >= (int64_t)a.d.P * a.d.B * nc) return;
+    const int row = (int)(i / nc), e = (int)(i % nc), c = e % a.d.C;
+    const float A = a.A[a.d.net[row / a.d.B] * nc + e] * LOG2E;
+    float h = start != nullptr ? start[i] : 0.f;
+#pragma unroll 4
+    for (int k = 0; k < a.nchunk; ++k) {
+        const int64_t at = (int64_t)row * a.nchunk + (reverse ? a.nchunk - 1 - k : k);
+        const float s = a.sums[at * a.d.C + c], own = a.carry[at * nc + e];
+        a.carry[at * nc + e] = h;
+        h = s == s ? fmaf(exp2_fast(A * s), h, own) : own;
+    }
+}
+
 // ---- backward --------------------------------------------------------------------------------------------------------------------------
 // G_t = C_t dys_t + exp(dt_{t+1} A) G_{t+1} (dys: dy through the gate); a chunk leaves exp(dt_t A) G_t of its first step.
 // CARRY pass of a split sequence: what a chunk leaves by itself, and its sum of dt.
-template <class T, int NS>
+template <class T, int NL, int NS>
 __global__ __launch_bounds__(256) void ssm_scan_bwd_carry_kernel(ScanArgs a) {
     constexpr int NP = NS * NL, KG = K / NS;
     __shared__ float lds[4][2][K * NP];
@@ -319,11 +381,12 @@ __global__ __launch_bounds__(256) void ssm_scan_bwd_carry_kernel(ScanArgs a) {
     if (item >= a.items) return;
     const int ncb = a.d.G * a.nblk, rc = uni(item / ncb), cb = item - rc * ncb;
     const int row = uni(rc / a.nchunk), ch = rc - row * a.nchunk, p = uni(row / a.d.B), b = row - p * a.d.B;
-    const Lane<T, NS> q(a, cb, threadIdx.x & 63);
+    const Lane<NL, NS> q(a, cb, threadIdx.x & 63);
     const int N = a.d.N, C = a.d.C, net = a.d.net[p], len = uni(seq_len(a.lengths, b, a.d.S)), lane = q.lane;
     const int first = ch * a.chunk, last = first + a.chunk < a.d.S ? first + a.chunk : a.d.S, end = len < last ? len : last;
-    const SeqPtr<T, NS> ds(a.delta, q, p, b), zs(a.z, q, p, b), gs(a.dy, q, p, b);
-    const T* Cp = seq_at<T>(a.Cm, p, b) + q.grp * N;
+    const int tl = first + (end - 1 - first) / K * K;  // the last block
+    SeqPtr<T, NS> ds(a.delta, q, p, b, tl), zs(a.z, q, p, b, tl), gs(a.dy, q, p, b, tl);
+    MapsPtr<T, NP, 64> ms(a, p, b, q.grp, tl, threadIdx.x & 63);
     const bool gated = a.z.data != nullptr;
     float A[NL], dh[NL];
     load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
@@ -339,18 +402,21 @@ __global__ __launch_bounds__(256) void ssm_scan_bwd_carry_kernel(ScanArgs a) {
 #pragma unroll
         for (int i = 0; i < KG; ++i) {
             const int out = behind(t0 + i * NS, q.g, end);
-            ds.load(dr[i], t0 + i * NS, out);
-            gs.load(gy[i], t0 + i * NS, out);
-            if (gated) zs.load(z[i], t0 + i * NS, out);
+            ds.load(dr[i], i * NS, out);
+            gs.load(gy[i], i * NS, out);
+            if (gated) zs.load(z[i], i * NS, out);
         }
-        maps.load(a, Cp, Cp, t0, end, lane);
+        ms.load(maps, t0, end, lane);
         rs = load_reset(a, b, t0, end, lane);
+        ds.move(-K);
+        zs.move(-K);
+        gs.move(-K);
+        ms.move(-K);
     };
-    const int tl = first + (end - 1 - first) / K * K;
     if (first < end) request(tl);
     for (int t0 = tl; t0 >= first && first < end; t0 -= K) {
         wave_lds_sync();
-        maps.store(lb, lc, lane);
+        store_maps(maps, lb, lc, lane);
         const unsigned fresh = reset_bits(rs);
         float dt[KG], dys[KG];
 #pragma unroll
@@ -375,9 +441,7 @@ __global__ __launch_bounds__(256) void ssm_scan_bwd_carry_kernel(ScanArgs a) {
                 const int s = i * NS + j;
 #pragma unroll
                 for (int n = 0; n < NL; ++n) dh[n] = fmaf(gys[j], lc[s * NP + q.n0 + n], dh[n]) * exp2_fast(dts[j] * A[n]);
-                if (fresh >> s & 1)
-#pragma unroll
-                    for (int n = 0; n < NL; ++n) dh[n] = 0.f;
+                if (fresh >> s & 1) clear(dh);
             }
         }
     }
@@ -401,7 +465,7 @@ __device__ __forceinline__ void put_map(const ScanArgs& a, float v, int64_t om, 
 
 // Blocks of K steps from the last to the first: a block's states are recomputed from its record into registers, then its steps run backwards.
 // A workgroup's waves own neighbouring channels of the same rows: they share B and C in LDS and add up their shares of dB and dC there.
-template <class T, int NS>
+template <class T, int NL, int NS>
 __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) {
     constexpr int NP = NS * NL, KG = K / NS, TOP = 32 / NS;
     __shared__ float lb[K * NP], lc[K * NP], red[WMAX][K][2 * NP];
@@ -410,7 +474,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
     const int gw = a.d.G * a.wgs, ps = uni((int)blockIdx.x / gw), wg = (int)blockIdx.x - ps * gw, p = uni(ps / a.slots), slot = ps - p * a.slots;
     const int grp = uni(wg / a.wgs), run = wg - grp * a.wgs;
     const int kblk = run * a.wpb + wv;  // may lie behind the last block: such a wave has no channels and only helps along
-    Lane<T, NS> q(a, grp * a.nblk + (kblk < a.nblk ? kblk : a.nblk - 1), threadIdx.x & 63);
+    Lane<NL, NS> q(a, grp * a.nblk + (kblk < a.nblk ? kblk : a.nblk - 1), threadIdx.x & 63);
     if (kblk >= a.nblk) q.act = false;
     const int N = a.d.N, C = a.d.C, S = a.d.S, NB = a.d.B, net = a.d.net[p], lane = q.lane;
     float A[NL], dA[NL];
@@ -428,8 +492,9 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
         const int b = uni(it / a.nchunk), ch = it - b * a.nchunk;
         const int row = p * NB + b, len = uni(seq_len(a.lengths, b, S));
         const int first = ch * a.chunk, last = first + a.chunk < S ? first + a.chunk : S, end = len < last ? len : last;
-        const SeqPtr<T, NS> xs(a.x, q, p, b), ds(a.delta, q, p, b), zs(a.z, q, p, b), gs(a.dy, q, p, b);
-        const T *Bp = seq_at<T>(a.Bm, p, b) + grp * N, *Cp = seq_at<T>(a.Cm, p, b) + grp * N;
+        const int tl = first + (end - 1 - first) / K * K;  // the last block
+        SeqPtr<T, NS> xs(a.x, q, p, b, tl), ds(a.delta, q, p, b, tl), zs(a.z, q, p, b, tl), gs(a.dy, q, p, b, tl);
+        MapsPtr<T, NP, 64> ms(a, p, b, grp, tl, lane);
         const int64_t o = ((int64_t)p * S * NB + b) * C + q.first, om = (((int64_t)p * S * NB + b) * a.d.G + grp) * N;
         const int64_t pm = om + (int64_t)run * a.d.P * S * NB * a.d.G * N;
         T *dxp = static_cast<T*>(a.dx) + o, *ddp = static_cast<T*>(a.ddelta) + o, *dzp = static_cast<T*>(a.dz) + o;
@@ -442,24 +507,29 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
             if (gated) row_store(0.f, dzp + t * yst, ROW_MAX, off);
             for (int i = threadIdx.x; i < 2 * NP; i += nthr) put_map<T, NP>(a, 0.f, om, pm, t * mst, i);
         }
-        for (int t0 = first + (end - 1 - first) / K * K; t0 >= first && first < end; t0 -= K) {
+        for (int t0 = tl; t0 >= first && first < end; t0 -= K) {
             Raw<T> xr[KG], dr[KG], zr[KG], gr[KG];
             Maps<T, NP, 64> maps;
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
                 const int out = behind(t0 + i * NS, q.g, end);
-                xs.load(xr[i], t0 + i * NS, out);
-                ds.load(dr[i], t0 + i * NS, out);
-                gs.load(gr[i], t0 + i * NS, out);
-                if (gated) zs.load(zr[i], t0 + i * NS, out);
+                xs.load(xr[i], i * NS, out);
+                ds.load(dr[i], i * NS, out);
+                gs.load(gr[i], i * NS, out);
+                if (gated) zs.load(zr[i], i * NS, out);
             }
             const int rs = load_reset(a, b, t0, end, lane);
             float hs[K + 1][NL];  // hs[s]: the state before step s; hs[K]: after the block
             load_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, 1.f, hs[0]);
             if (wv == 0) {
-                maps.load(a, Bp, Cp, t0, end, lane);
-                maps.store(lb, lc, lane);
+                ms.load(maps, t0, end, lane);
+                store_maps(maps, lb, lc, lane);
             }
+            xs.move(-K);
+            ds.move(-K);
+            zs.move(-K);
+            gs.move(-K);
+            ms.move(-K);
             __syncthreads();
             const unsigned fresh = reset_bits(rs);
             float x[KG], dt[KG], dys[KG], sd[KG];  // sd: the step size's slope
@@ -479,9 +549,11 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                     // a reset empties the state through the decay, e^-inf = 0; what is not finite has to go by hand
                     const bool re = fresh >> s & 1;
                     const float fr = re ? -INFINITY : 0.f;
-                    if (re)
+                    if (re) {
+                        asm volatile("");
 #pragma unroll
                         for (int n = 0; n < NL; ++n) hs[s][n] = fabsf(hs[s][n]) < INFINITY ? hs[s][n] : 0.f;
+                    }
                     float y = 0.f;
 #pragma unroll
                     for (int n = 0; n < NL; ++n) {
@@ -525,16 +597,11 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                         sa = fmaf(w, A[n], sa);
                         dA[n] = fmaf(w, dts[j], dA[n]);
                     };
-                    float sum = pair_tree<TOP, 3, 0>(state, lane);
-                    if constexpr (NS == 1) sum += dpp_xor3(sum);
-                    if constexpr (NS <= 2) sum += dpp_xor1(sum);
+                    const float sum = pair_sums<NL, TOP>(state, lane);
                     gb[j] = sb;
                     ga[j] = sa;
-                    if (re)
-#pragma unroll
-                        for (int n = 0; n < NL; ++n) dh[n] = 0.f;
-                    // lane bit TOP: dB / dC, the three below: n (within the lane's group)
-                    red[wv][s][(lane / TOP & 1) * NP + q.n0 + (lane / (TOP / 8) & 7)] = sum;
+                    if (re) clear(dh);
+                    red[wv][s][(lane / TOP & 1) * NP + q.n0 + (lane / (TOP / NL) & (NL - 1))] = sum;
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 const int out = behind(t1 + i * NS, q.g, end);
@@ -595,29 +662,41 @@ int scan_validate(const marlhip_ssm_shape* s) {
 }
 
 struct ScanPlan {
-    int NS, nblk, chunk, nchunk, nck, wpb, wgs, slots;
+    int NL, NS, nblk, chunk, nchunk, nck, wpb, wgs, slots;
 };
 
-// How a call is split.  One wave a SIMD (1024 of them) is where the chip begins to be filled; a sequence of fewer is worth cutting into chunks,
-// which costs a first pass over delta, x and B (or dy, C) of about 0.8 of the second one: below half of that number only.
+// How a call is split.  One wave a SIMD (1024 of them) is where the chip begins to be filled.  Batches that stay below keep 4 states a lane
+// instead of 8 (twice the waves for a sixth more instructions); a sequence of still fewer is cut into chunks, which costs a first pass over
+// delta, x and B (or dy, C) of about 0.8 of the second one.
 ScanPlan scan_plan(const marlhip_ssm_shape* s) {
+    static const int TGT = getenv("SSM_T") ? atoi(getenv("SSM_T")) : 4096, THR = getenv("SSM_H") ? atoi(getenv("SSM_H")) : 512, MINC = getenv("SSM_C") ? atoi(getenv("SSM_C")) : 64;
+    static const int WM = getenv("SSM_W") ? atoi(getenv("SSM_W")) : WMAX;
+    static const int N4 = getenv("SSM_N4") ? atoi(getenv("SSM_N4")) : 1024;
     ScanPlan q;
-    q.NS = scan_np(s->state) / NL;
-    const int CL = 64 / q.NS;
-    q.nblk = (s->channels / s->groups + CL - 1) / CL;
+    const int Cg = s->channels / s->groups;
+    auto lanes = [&](int nl, int ns) {
+        q.NL = nl;
+        q.NS = ns;
+        q.nblk = (Cg + 64 / ns - 1) / (64 / ns);
+        return (int64_t)s->n_agents * s->batch * s->groups * q.nblk;
+    };
+    int64_t waves;
+    if (s->state <= 4) waves = lanes(4, 1);
+    else if (s->state <= 8) waves = lanes(8, 1) <= N4 ? lanes(4, 2) : lanes(8, 1);
+    else if (s->state <= 16) waves = lanes(8, 2) <= N4 ? lanes(4, 4) : lanes(8, 2);
+    else waves = lanes(8, 4);
     q.nck = (s->steps + K - 1) / K;
-    const int64_t waves = (int64_t)s->n_agents * s->batch * s->groups * q.nblk;
     q.nchunk = 1;
     q.chunk = q.nck > 0 ? q.nck * K : K;
-    if (waves > 0 && waves <= 512 && s->steps >= 128) {
-        int64_t want = 2048 / waves, most = s->steps / 64;
+    if (waves > 0 && waves <= THR && s->steps >= 2 * MINC) {
+        int64_t want = TGT / waves, most = s->steps / MINC;
         if (want > most) want = most;
         if (want > 1) {
             q.chunk = (int)((q.nck + want - 1) / want) * K;
             q.nchunk = (s->steps + q.chunk - 1) / q.chunk;
         }
     }
-    q.wpb = q.nblk < WMAX ? q.nblk : WMAX;
+    q.wpb = q.nblk < WM ? q.nblk : WM;
     q.wgs = (q.nblk + q.wpb - 1) / q.wpb;
     // items of one agent that a backward workgroup takes one after the other (its sums over them stay in registers)
     const int64_t items = (int64_t)s->batch * q.nchunk, k = 4096 / ((int64_t)s->n_agents * s->groups * q.wgs * q.wpb);
@@ -637,6 +716,8 @@ int scan_seqs(const char* what, const marlhip_ssm_shape* s, const marlhip_ssm_sc
     const int e = s->dtype == 0 ? 4 : 2;
     if (seq_check(what, "x", q->x, e, s->steps) || seq_check(what, "delta", q->delta, e, s->steps) || seq_check(what, "z", q->z, e, s->steps)) return -1;
     if (grad && seq_check(what, "dy", q->dy, e, s->steps)) return -1;
+    // the maps' offsets run over K steps: half the span
+    if (seq_check(what, "B", q->B, 2 * e, s->steps) || seq_check(what, "C", q->C, 2 * e, s->steps)) return -1;
     MARL_REQUIRE(scan_items(s, scan_plan(s)) < (1ll << 31) - 8, "%s: batch %d x channels %d is too large", what, s->batch, s->channels);
     MARL_REQUIRE(s->steps <= 1 || (int64_t)s->batch * s->channels * e <= (1ll << 29), "%s: batch %d x channels %d: a step is over 2^29 bytes", what, s->batch,
                  s->channels);
@@ -658,17 +739,23 @@ ScanArgs scan_args(const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q, c
 
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// f(type, lanes a channel)
+// f(type, states a lane, lanes a channel)
 template <class F>
-void by_type_and_state(const marlhip_ssm_shape* s, int NS, F f) {
-    auto by_ns = [&](auto t) {
-        if (NS == 1) f(t, Idx<1>{});
-        else if (NS == 2) f(t, Idx<2>{});
-        else f(t, Idx<4>{});
+void by_type_and_lanes(const marlhip_ssm_shape* s, const ScanPlan& pl, F f) {
+    auto by_lanes = [&](auto t) {
+        if (pl.NL == 8) {
+            if (pl.NS == 1) f(t, Idx<8>{}, Idx<1>{});
+            else if (pl.NS == 2) f(t, Idx<8>{}, Idx<2>{});
+            else f(t, Idx<8>{}, Idx<4>{});
+        } else {
+            if (pl.NS == 1) f(t, Idx<4>{}, Idx<1>{});
+            else if (pl.NS == 2) f(t, Idx<4>{}, Idx<2>{});
+            else f(t, Idx<4>{}, Idx<4>{});
+        }
     };
-    if (s->dtype == 0) by_ns(float{});
-    else if (s->dtype == 1) by_ns(__bf16{});
-    else by_ns(_Float16{});
+    if (s->dtype == 0) by_lanes(float{});
+    else if (s->dtype == 1) by_lanes(__bf16{});
+    else by_lanes(_Float16{});
 }
 
 struct CarryWs {
@@ -684,6 +771,13 @@ CarryWs carry_ws(const marlhip_ssm_shape* s, const ScanPlan& pl) {
 }
 
 int join(const ScanArgs& a, const float* start, int reverse, hipStream_t st) {
+    if (a.nchunk <= 16) {
+        const int64_t wgs = ((int64_t)a.d.P * a.d.B * a.d.N * a.d.C + 255) / 256;
+        MARL_REQUIRE(wgs < (1ll << 31), "ssm_scan: too many rows");
+        hipLaunchKernelGGL(ssm_scan_join_few_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a, start, reverse);
+        MARL_CHECK_LAUNCH("ssm_scan_join_few_kernel");
+        return 0;
+    }
     const int64_t wgs = (int64_t)a.d.P * a.d.B * a.d.N * ((a.d.C + 63) / 64);
     MARL_REQUIRE(wgs < (1ll << 31), "ssm_scan: too many rows");
     hipLaunchKernelGGL(ssm_scan_join_kernel, dim3((unsigned)wgs), dim3(1024), 0, st, a, start, reverse);
@@ -721,14 +815,14 @@ extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_sc
     if (pl.nchunk > 1) {
         a.carry = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.carry);
         a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.sums);
-        by_type_and_state(s, pl.NS, [&](auto t, auto ns) {
-            hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(ns)::v, true>), grid, dim3(256), 0, st, a);
+        by_type_and_lanes(s, pl, [&](auto t, auto nl, auto ns) {
+            hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v, true>), grid, dim3(256), 0, st, a);
         });
         MARL_CHECK_LAUNCH("ssm_scan_fwd_kernel");
         if (join(a, a.h_in, 0, st) != 0) return -2;
     }
-    by_type_and_state(s, pl.NS, [&](auto t, auto ns) {
-        hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(ns)::v, false>), grid, dim3(256), 0, st, a);
+    by_type_and_lanes(s, pl, [&](auto t, auto nl, auto ns) {
+        hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v, false>), grid, dim3(256), 0, st, a);
     });
     MARL_CHECK_LAUNCH("ssm_scan_fwd_kernel");
     return 0;
@@ -783,14 +877,14 @@ extern "C" int marlhip_ssm_scan_grad(const marlhip_ssm_shape* s, const marlhip_s
         a.sums = reinterpret_cast<float*>(ws + w.carry.sums);
         a.items = (int)scan_items(s, pl);
         const dim3 grid((unsigned)((a.items + 3) / 4));
-        by_type_and_state(s, pl.NS, [&](auto t, auto ns) {
-            hipLaunchKernelGGL((ssm_scan_bwd_carry_kernel<decltype(t), decltype(ns)::v>), grid, dim3(256), 0, st, a);
+        by_type_and_lanes(s, pl, [&](auto t, auto nl, auto ns) {
+            hipLaunchKernelGGL((ssm_scan_bwd_carry_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v>), grid, dim3(256), 0, st, a);
         });
         MARL_CHECK_LAUNCH("ssm_scan_bwd_carry_kernel");
         if (join(a, a.dh_out, 1, st) != 0) return -2;
     }
     const dim3 grid((unsigned)(s->n_agents * pl.slots * s->groups * pl.wgs)), block(64 * pl.wpb);
-    by_type_and_state(s, pl.NS, [&](auto t, auto ns) { hipLaunchKernelGGL((ssm_scan_bwd_kernel<decltype(t), decltype(ns)::v>), grid, block, 0, st, a); });
+    by_type_and_lanes(s, pl, [&](auto t, auto nl, auto ns) { hipLaunchKernelGGL((ssm_scan_bwd_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v>), grid, block, 0, st, a); });
     MARL_CHECK_LAUNCH("ssm_scan_bwd_kernel");
     const int64_t maps = (int64_t)s->n_agents * s->steps * s->batch * s->groups * s->state;
     if (pl.wgs > 1 && maps > 0) {
@@ -803,7 +897,7 @@ extern "C" int marlhip_ssm_scan_grad(const marlhip_ssm_shape* s, const marlhip_s
         MARL_CHECK_LAUNCH("ssm_maps_sum_kernel");
     }
     const int64_t cols = (int64_t)(s->state + 2) * s->channels;
-    hipLaunchKernelGGL(ssm_weights_sum_kernel, dim3((unsigned)((cols + 63) / 64), a.d.M), dim3(256), 0, st, a.d, pl.slots, s->state, 2, a.part, q->dA, q->dD,
+    hipLaunchKernelGGL(ssm_weights_sum_kernel, dim3((unsigned)((cols + 63) / 64), a.d.M), dim3(1024), 0, st, a.d, pl.slots, s->state, 2, a.part, q->dA, q->dD,
                        q->ddelta_bias);
     MARL_CHECK_LAUNCH("ssm_weights_sum_kernel");
     return 0;
