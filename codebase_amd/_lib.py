@@ -271,17 +271,19 @@ PROTOTYPES = {
                                                 c_void_p, c_void_p, c_void_p]),
     "marlhip_idqn_update_n_split16": (c_int32, [POINTER(IdqnLearner), c_int32, c_int32, c_uint64, c_uint32, POINTER(c_int64),
                                                 POINTER(c_int64), POINTER(c_int64), c_void_p]),
-    "marlhip_ssm_conv": (c_int32, [POINTER(SsmShape), POINTER(SsmConvArgs), c_void_p]),
-    "marlhip_ssm_conv_grad_workspace_bytes": (c_int64, [POINTER(SsmShape)]),
-    "marlhip_ssm_conv_grad": (c_int32, [POINTER(SsmShape), POINTER(SsmConvArgs), c_void_p, c_int64, c_void_p]),
-    "marlhip_ssm_scan_record_floats": (c_int64, [POINTER(SsmShape)]),
-    "marlhip_ssm_scan_workspace_bytes": (c_int64, [POINTER(SsmShape)]),
-    "marlhip_ssm_scan": (c_int32, [POINTER(SsmShape), POINTER(SsmScanArgs), c_void_p, c_int64, c_void_p]),
-    "marlhip_ssm_scan_grad_workspace_bytes": (c_int64, [POINTER(SsmShape)]),
-    "marlhip_ssm_scan_grad": (c_int32, [POINTER(SsmShape), POINTER(SsmScanArgs), c_void_p, c_int64, c_void_p]),
-    "marlhip_grad_norm_workspace_bytes": (c_int64, [POINTER(TensorStruct), c_int32]),
-    "marlhip_grad_norm": (c_int32, [POINTER(TensorStruct), c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
-    "marlhip_clip_grad_norm": (c_int32, [POINTER(TensorStruct), c_int32, c_float, c_void_p, c_void_p, c_int64, c_void_p]),
+    # (shape and argument structs as packed bytes or byref of the classes above; marlhip_tensor arrays by address: hip.py)
+    "marlhip_ssm_conv": (c_int32, [c_void_p, c_void_p, c_void_p]),
+    "marlhip_ssm_conv_grad_workspace_bytes": (c_int64, [c_void_p]),
+    "marlhip_ssm_conv_grad": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "marlhip_ssm_scan_record_floats": (c_int64, [c_void_p]),
+    "marlhip_ssm_scan_workspace_bytes": (c_int64, [c_void_p]),
+    "marlhip_ssm_scan": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "marlhip_ssm_scan_grad_workspace_bytes": (c_int64, [c_void_p]),
+    "marlhip_ssm_scan_grad": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "marlhip_tensors_apart": (c_int32, [c_void_p, c_int32]),
+    "marlhip_grad_norm_workspace_bytes": (c_int64, [c_void_p, c_int32]),
+    "marlhip_grad_norm": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
+    "marlhip_clip_grad_norm": (c_int32, [c_void_p, c_int32, c_float, c_void_p, c_void_p, c_int64, c_void_p]),
     "marlhip_timing_enable": (c_int32, [c_int32]),
     "marlhip_timing_read": (c_int32, [c_int32, POINTER(c_int64), POINTER(c_double)]),
     "marlhip_idqn_collect": (c_int32, [POINTER(LbfConfig), POINTER(NetShape), c_void_p, c_float, c_uint32,

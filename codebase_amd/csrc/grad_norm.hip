@@ -3,6 +3,9 @@
 // The tensors' pointers travel in the kernel's own arguments, up to NORM_ENTRIES a launch: no table has to be copied to the device, and a
 // captured graph holds them.  A first pass leaves one 64-bit sum of squares a workgroup, a second one adds them up in every workgroup (the
 // same order everywhere) and scales.  Bound by HBM: the gradients are read once or twice and written once.
+#include <algorithm>
+#include <vector>
+
 #include "common.h"
 
 using namespace marl;
@@ -210,6 +213,32 @@ int norm_check(const marlhip_tensor* t, int32_t count, NormPlan& plan, void* wor
 }
 
 }  // namespace
+
+extern "C" int marlhip_tensors_apart(const marlhip_tensor* t, int32_t count) {
+    MARL_REQUIRE(count >= 0 && (count == 0 || t != nullptr), "tensors_apart: %d tensors", count);
+    struct Span {
+        uintptr_t lo, hi;
+        int i;
+    };
+    // caught here: no exception may leave a C entry point
+    try {
+        std::vector<Span> v;
+        v.reserve(2 * (size_t)count);
+        for (int i = 0; i < count; ++i) {
+            const uintptr_t n = (uintptr_t)t[i].n * (t[i].dtype == 0 ? 4 : 2), p = (uintptr_t)t[i].data, o = t[i].out != nullptr ? (uintptr_t)t[i].out : p;
+            if (n == 0) continue;
+            v.push_back({p, p + n, i});
+            if (o != p) v.push_back({o, o + n, i});
+        }
+        std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+        for (size_t k = 1; k < v.size(); ++k)
+            MARL_REQUIRE(v[k - 1].hi <= v[k].lo, "tensors %d and %d overlap", v[k - 1].i, v[k].i);
+    } catch (...) {
+        set_error("tensors_apart: out of memory");
+        return -1;
+    }
+    return 0;
+}
 
 extern "C" int64_t marlhip_grad_norm_workspace_bytes(const marlhip_tensor* tensors, int32_t count) {
     NormPlan plan;

@@ -507,9 +507,11 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
             if (gated) row_store(0.f, dzp + t * yst, ROW_MAX, off);
             for (int i = threadIdx.x; i < 2 * NP; i += nthr) put_map<T, NP>(a, 0.f, om, pm, t * mst, i);
         }
-        for (int t0 = tl; t0 >= first && first < end; t0 -= K) {
-            Raw<T> xr[KG], dr[KG], zr[KG], gr[KG];
-            Maps<T, NP, 64> maps;
+        Raw<T> xr[KG], dr[KG], zr[KG], gr[KG];
+        Maps<T, NP, 64> maps;
+        int rs;
+        float hb[NL];  // the state the block starts from
+        auto request = [&](int t0) __attribute__((always_inline)) {  // the pointers are at t0
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
                 const int out = behind(t0 + i * NS, q.g, end);
@@ -518,28 +520,38 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                 gs.load(gr[i], i * NS, out);
                 if (gated) zs.load(zr[i], i * NS, out);
             }
-            const int rs = load_reset(a, b, t0, end, lane);
-            float hs[K + 1][NL];  // hs[s]: the state before step s; hs[K]: after the block
-            load_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, 1.f, hs[0]);
-            if (wv == 0) {
-                ms.load(maps, t0, end, lane);
-                store_maps(maps, lb, lc, lane);
-            }
+            rs = load_reset(a, b, t0, end, lane);
+            load_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, 1.f, hb);
+            if (wv == 0) ms.load(maps, t0, end, lane);
             xs.move(-K);
             ds.move(-K);
             zs.move(-K);
             gs.move(-K);
             ms.move(-K);
-            __syncthreads();
+        };
+        if (first < end) request(tl);
+        for (int t0 = tl; t0 >= first && first < end; t0 -= K) {
+            float hs[K + 1][NL];                       // hs[s]: the state before step s; hs[K]: after the block
+            float x[KG], dt[KG], dys[KG], sd[KG], zv[KG];  // sd: the step size's slope
+            if (wv == 0) store_maps(maps, lb, lc, lane);
             const unsigned fresh = reset_bits(rs);
-            float x[KG], dt[KG], dys[KG], sd[KG];  // sd: the step size's slope
+#pragma unroll
+            for (int n = 0; n < NL; ++n) hs[0][n] = hb[n];
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
-                const int out = behind(t0 + i * NS, q.g, end);  // a step behind the end changes nothing: dt = 0, x = 0, dy = 0
                 const float raw = dr[i].get() + bias;
                 x[i] = xr[i].get();
-                dt[i] = out ? 0.f : (a.softplus ? softplus(raw) : raw);
+                dys[i] = gr[i].get();
+                zv[i] = gated ? zr[i].get() : 0.f;
+                // a step behind the end changes nothing: dt = 0, x = 0, dy = 0
+                dt[i] = behind(t0 + i * NS, q.g, end) ? 0.f : (a.softplus ? softplus(raw) : raw);
                 sd[i] = a.softplus ? sigmoid(raw) : 1.f;
+            }
+            __syncthreads();
+            if (t0 > first) request(t0 - K);
+#pragma unroll
+            for (int i = 0; i < KG; ++i) {
+                const int out = behind(t0 + i * NS, q.g, end);
                 float dts[NS], us[NS], ys[NS];
                 to_groups<NS>(dt[i], dts);
                 to_groups<NS>(dt[i] * x[i], us);
@@ -563,9 +575,8 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                     ys[j] = y;
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                dys[i] = gr[i].get();
                 if (gated) {
-                    const float y = fmaf(D, x[i], from_groups<NS>(ys)), z = zr[i].get(), sg = sigmoid(z);
+                    const float y = fmaf(D, x[i], from_groups<NS>(ys)), z = zv[i], sg = sigmoid(z);
                     row_store(dys[i] * y * sg * fmaf(z, 1.f - sg, 1.f), dzp + (t0 + i * NS) * yst, ROW_MAX, yoff | out);
                     dys[i] *= z * sg;
                 }

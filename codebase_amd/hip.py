@@ -1,7 +1,9 @@
 """Tensor-level Python face of libmarlhip.so: PyTorch-ROCm tensors in, kernels enqueued on the
 current torch stream, nothing copied to the host.  torch is plumbing here (device memory,
 streams); every computation below happens in the HIP library."""
+import array
 import ctypes
+import struct
 from collections import namedtuple
 from dataclasses import dataclass
 
@@ -10,8 +12,7 @@ import torch
 import os
 
 from . import _lib
-from ._lib import (AcConfig, BatchStruct, IdqnLearner, QmixLearner, RetStatsStruct, QmixMixer, LbfBuffers, LbfConfig, MarlHipError, RwareConfig, NetShape, ReplayBuffers, ReplayShape, SsmConvArgs, SsmScanArgs, SsmSeq,
-                   SsmShape, TensorStruct, check, lib)
+from ._lib import (AcConfig, BatchStruct, IdqnLearner, QmixLearner, RetStatsStruct, QmixMixer, LbfBuffers, LbfConfig, MarlHipError, RwareConfig, NetShape, ReplayBuffers, ReplayShape, check, lib)
 
 Batch = namedtuple("Batch", ["obss", "actions", "rewards", "dones", "filled", "action_mask"])  # dqn/train.py:14-16
 
@@ -1324,115 +1325,134 @@ def sample_from_logits(logits, seed, episode, t):
 # Sequences are [P][S][B][C] tensors (agents, steps, batch, channels) as everywhere; x / delta / z / dy and the maps B / C [P][S][B][G][N] may
 # be slices of wider projections or expanded, as long as the last dimension (for the maps the last two) is dense.  f32, bf16 or f16, one type
 # per call; weights, their gradients and the scan's state are f32.
+#
+# An acting step is a few microseconds of GPU time, so the way to the launch is kept short: a tensor is checked by one expression (the slow
+# _expect only words the refusal), the C structs are packed at once, sizes that depend on the shape alone are kept by shape.
 
 _SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F32 = torch.float32
 
 SsmConvGrad = namedtuple("SsmConvGrad", ["x", "weight", "bias", "state"])
 SsmScanGrad = namedtuple("SsmScanGrad", ["x", "delta", "A", "B", "C", "D", "z", "delta_bias", "h_in"])
 
+# include/marlhip.h: marlhip_ssm_shape, marlhip_ssm_conv_args, marlhip_ssm_scan_args (pointers as unsigned 64-bit words, NULL = 0)
+_SHAPE_PACK = struct.Struct("=24i").pack
+_CONV_PACK = struct.Struct("=" + "Qqqq" * 2 + "QQi4x" + "Q" * 10).pack
+_SCAN_PACK = struct.Struct("=" + "Qqqq" * 6 + "QQQi4x" + "Q" * 16).pack
+_NO_SEQ = (0, 0, 0, 0)
+_SSM_SIZES = {}  # (what, shape struct) -> bytes or floats
 
-def _expect(what, name, t, shape, dtype, device, dense=True):
-    """argument checks of the sequence operators: ValueError names the tensor (None passes: optional arguments)"""
-    if t is None:
-        return
+
+def _expect(what, name, t, shape, dtype, dev, dense=True):
+    """the refusal of an argument that did not pass: ValueError names the tensor and what is wrong with it"""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what}: {name} is not a tensor")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{what}: {name} is {t.dtype}, expected {dtype}")
-    if t.device != device:
-        raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}, expected {'the CPU' if dev < 0 else f'cuda:{dev}'}")
     if dense and not t.is_contiguous():
         raise ValueError(f"{what}: {name} is not contiguous")
 
 
-def _expect_seq(what, name, t, shape, dtype, device):
-    _expect(what, name, t, shape, dtype, device, dense=False)
-    if t is None or t.numel() == 0:
-        return
-    step = 1
-    for d in range(t.dim() - 1, 2, -1):  # channels, or a map's groups and states
-        if t.shape[d] != 1 and t.stride(d) != step:
-            raise ValueError(f"{what}: {name} has stride {t.stride(d)} in dimension {d}, expected {step}")
-        step *= t.shape[d]
+def _dense(what, name, t, shape, dtype, dev):
+    """address of a contiguous argument (0: absent)"""
+    if t is None:
+        return 0
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        _expect(what, name, t, shape, dtype, dev)
+    return t.data_ptr()
 
 
-def _seq(t):
-    return SsmSeq() if t is None else SsmSeq(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+def _seq(what, name, t, shape, dtype, dev):
+    """marlhip_ssm_seq of a sequence or a map"""
+    if t is None:
+        return _NO_SEQ
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+        _expect(what, name, t, shape, dtype, dev, dense=False)
+    st = t.stride()
+    if st[-1] != 1 or len(shape) == 5:
+        step = 1
+        for d in range(len(shape) - 1, 2, -1):  # channels, or a map's groups and states
+            if shape[d] != 1 and st[d] != step and t.numel():
+                raise ValueError(f"{what}: {name} has stride {st[d]} in dimension {d}, expected {step}")
+            step *= shape[d]
+    return t.data_ptr(), st[0], st[1], st[2]
 
 
 def _ssm_shape(what, x, state, groups, sharing):
-    """shape struct of a call, and its number of networks"""
+    """packed marlhip_ssm_shape of a call, its number of networks and the device (-1: CPU)"""
     if not isinstance(x, torch.Tensor) or x.dim() != 4:
         raise ValueError(f"{what}: x is not a [agents][steps][batch][channels] tensor")
-    if x.dtype not in _SEQ_DTYPES:
+    code = _SEQ_DTYPES.get(x.dtype)
+    if code is None:
         raise ValueError(f"{what}: {x.dtype} is not supported (float32, bfloat16, float16)")
     P, S, B, C = x.shape
-    s = SsmShape(P, S, B, C, int(state), int(groups), _SEQ_DTYPES[x.dtype], 0)
     if sharing is None:
-        return s, P
+        return _SHAPE_PACK(P, S, B, C, state, groups, code, 0, *_NO_NETS), P, x.get_device()
     if len(sharing) != P or P > 16:
         raise ValueError(f"{what}: sharing indices: one per agent, at most 16 agents")
-    s.n_networks = max(sharing) + 1
-    for i, k in enumerate(sharing):
-        s.net_of[i] = int(k)
-    return s, s.n_networks
+    M = max(sharing) + 1
+    return _SHAPE_PACK(P, S, B, C, state, groups, code, M, *sharing, *_NO_NETS[P:]), M, x.get_device()
 
 
-def _episode_flags(what, x, reset, lengths):
-    S, B = x.shape[1:3]
+_NO_NETS = (0,) * 16
+
+
+def _ssm_size(fn, what, shape):
+    """a size that depends on the shape alone"""
+    n = _SSM_SIZES.get((what, shape))
+    if n is None:
+        n = check(fn(shape), what)
+        if len(_SSM_SIZES) > 4096:
+            _SSM_SIZES.clear()
+        _SSM_SIZES[what, shape] = n
+    return n
+
+
+def _episode_flags(what, x, reset, lengths, dev):
+    """addresses of reset [S][B] and lengths [B]"""
+    _, S, B, _ = x.shape
     if reset is not None and isinstance(reset, torch.Tensor) and reset.dtype == torch.bool:
         reset = reset.view(torch.uint8)
-    _expect(what, "reset", reset, (S, B), torch.uint8, x.device)
-    _expect(what, "lengths", lengths, (B,), torch.int32, x.device)
-    return reset, lengths
+    return _dense(what, "reset", reset, (S, B), torch.uint8, dev), _dense(what, "lengths", lengths, (B,), torch.int32, dev)
 
 
 def _in_place_or_apart(what, name, out, src):
     """a carried state is updated in place or written elsewhere, not half over itself"""
-    if out is None or src is None or out.data_ptr() == src.data_ptr():
+    if out is None or src is None:
         return
-    a, b = out.data_ptr(), src.data_ptr()
-    n = out.numel() * out.element_size()
-    if a < b + n and b < a + n:
+    a, b, n = out.data_ptr(), src.data_ptr(), out.numel() * out.element_size()
+    if a != b and a < b + n and b < a + n:
         raise ValueError(f"{what}: {name} overlaps the state that the call reads")
 
 
-class _on_device:
-    """the device of the call's tensors, made current for its launches (the stream is that device's current one)"""
-
-    def __init__(self, x):
-        self.guard = torch.cuda.device(x.device)
-
-    def __enter__(self):
-        self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        return self.guard.__exit__(*exc)
+def _launch(what, dev, call):
+    """call(raw stream) with the tensors' device current: on that device's current stream"""
+    if torch._C._cuda_getDevice() == dev:
+        return call(torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return call(torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _need_device(what, x):
-    if x.device.type != "cuda":
-        raise MarlHipError(f"{what}: x is on {x.device}: marlhip needs tensors on an AMD GPU, there is no CPU path")
-    _require_gpu()
+def _need_device(what, t, dev):
+    if dev < 0:
+        raise MarlHipError(f"{what}: {'x' if what.startswith('ssm') else 'tensor 0'} is on {t.device}: marlhip needs tensors on an AMD GPU, there is no CPU path")
 
 
-def _conv_args(what, x, weight, bias, silu, sharing, state, reset, lengths):
+def _conv_args(what, x, weight, bias, sharing, state, reset, lengths):
+    """checked arguments: packed shape, device, addresses, shape of the window"""
     if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
         raise ValueError(f"{what}: weight is not a [networks][taps][channels] tensor")
     W = weight.shape[1]
-    s, M = _ssm_shape(what, x, W, 1, sharing)
-    P, S, B, C = x.shape
-    _expect_seq(what, "x", x, (P, S, B, C), x.dtype, x.device)
-    _expect(what, "weight", weight, (M, W, C), torch.float32, x.device)
-    _expect(what, "bias", bias, (M, C), torch.float32, x.device)
-    _expect(what, "state", state, (P, B, W - 1, C), x.dtype, x.device)
-    reset, lengths = _episode_flags(what, x, reset, lengths)
-    a = SsmConvArgs()
-    a.x, a.weight, a.bias, a.silu = _seq(x), _ptr(weight), _ptr(bias), int(bool(silu))
-    a.state, a.reset, a.lengths = _ptr(state), _ptr(reset), _ptr(lengths)
-    return s, a, (P, B, W - 1, C)
+    shape, M, dev = _ssm_shape(what, x, W, 1, sharing)
+    P, _, B, C = x.shape
+    window = (P, B, W - 1, C)
+    return (shape, dev, _seq(what, "x", x, x.shape, x.dtype, dev), _dense(what, "weight", weight, (M, W, C), _F32, dev),
+            _dense(what, "bias", bias, (M, C), _F32, dev), _dense(what, "state", state, window, x.dtype, dev),
+            *_episode_flags(what, x, reset, lengths, dev), window)
 
 
 def ssm_conv(x, weight, bias=None, silu=True, sharing=None, state=None, want_state=False, state_out=None, reset=None, lengths=None):
@@ -1441,69 +1461,63 @@ def ssm_conv(x, weight, bias=None, silu=True, sharing=None, state=None, want_sta
     (None: one each).  `state` [P][B][W-1][C]: the inputs before step 0 (None: zeros); `want_state` returns the ones after the last step, or
     `state_out` receives them (`state` itself: updated in place).  `reset` u8/bool [S][B]: an episode starts at this step, nothing before it
     is seen; `lengths` i32 [B]: steps of a row, those behind are not read and give 0.  -> y, or (y, state_out)"""
-    s, a, sshape = _conv_args("ssm_conv", x, weight, bias, silu, sharing, state, reset, lengths)
-    _expect("ssm_conv", "state_out", state_out, sshape, x.dtype, x.device)
+    shape, dev, xs, w, b, st, rs, ln, window = _conv_args("ssm_conv", x, weight, bias, sharing, state, reset, lengths)
+    so = _dense("ssm_conv", "state_out", state_out, window, x.dtype, dev)
     _in_place_or_apart("ssm_conv", "state_out", state_out, state)
-    _need_device("ssm_conv", x)
-    with _on_device(x):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if want_state and state_out is None:
-            state_out = torch.empty(sshape, dtype=x.dtype, device=x.device)
-        a.y, a.state_out = _ptr(y), _ptr(state_out)
-        check(lib.marlhip_ssm_conv(ctypes.byref(s), ctypes.byref(a), _stream()), "ssm_conv")
+    _need_device("ssm_conv", x, dev)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if want_state and state_out is None:
+        state_out = torch.empty(window, dtype=x.dtype, device=x.device)
+        so = state_out.data_ptr()
+    args = _CONV_PACK(*xs, *_NO_SEQ, w, b, 1 if silu else 0, st, rs, ln, y.data_ptr(), so, 0, 0, 0, 0, 0)
+    if _launch("ssm_conv", dev, lambda stream: lib.marlhip_ssm_conv(shape, args, stream)) < 0:
+        check(-1, "ssm_conv")
     return (y, state_out) if want_state else y
 
 
 def ssm_conv_grad(dy, x, weight, bias=None, silu=True, sharing=None, state=None, reset=None, lengths=None, dstate_out=None):
     """gradients of ssm_conv for the same arguments: dy [P][S][B][C] at y and (optional) dstate_out [P][B][W-1][C] at state_out ->
     SsmConvGrad(x, weight, bias, state); bias / state are None where the argument is"""
-    s, a, sshape = _conv_args("ssm_conv_grad", x, weight, bias, silu, sharing, state, reset, lengths)
-    _expect_seq("ssm_conv_grad", "dy", dy, x.shape, x.dtype, x.device)
-    _expect("ssm_conv_grad", "dstate_out", dstate_out, sshape, x.dtype, x.device)
-    _need_device("ssm_conv_grad", x)
-    with _on_device(x):
-        g = SsmConvGrad(torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight),
-                        None if bias is None else torch.empty_like(bias), None if state is None else torch.empty_like(state))
-        a.dy, a.dstate_out = _seq(dy), _ptr(dstate_out)
-        a.dx, a.dweight, a.dbias, a.dstate = _ptr(g.x), _ptr(g.weight), _ptr(g.bias), _ptr(g.state)
-        n = check(lib.marlhip_ssm_conv_grad_workspace_bytes(ctypes.byref(s)), "ssm_conv_grad_workspace_bytes")
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        check(lib.marlhip_ssm_conv_grad(ctypes.byref(s), ctypes.byref(a), _ptr(ws), n, _stream()), "ssm_conv_grad")
+    shape, dev, xs, w, b, st, rs, ln, window = _conv_args("ssm_conv_grad", x, weight, bias, sharing, state, reset, lengths)
+    dys = _seq("ssm_conv_grad", "dy", dy, x.shape, x.dtype, dev)
+    dso = _dense("ssm_conv_grad", "dstate_out", dstate_out, window, x.dtype, dev)
+    _need_device("ssm_conv_grad", x, dev)
+    n = _ssm_size(lib.marlhip_ssm_conv_grad_workspace_bytes, "ssm_conv_grad_workspace_bytes", shape)
+    g = SsmConvGrad(torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight),
+                    None if bias is None else torch.empty_like(bias), None if state is None else torch.empty_like(state))
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    args = _CONV_PACK(*xs, *dys, w, b, 1 if silu else 0, st, rs, ln, 0, 0, dso, *(0 if t is None else t.data_ptr() for t in (g.x, g.state, g.weight, g.bias)))
+    if _launch("ssm_conv_grad", dev, lambda stream: lib.marlhip_ssm_conv_grad(shape, args, ws.data_ptr(), n, stream)) < 0:
+        check(-1, "ssm_conv_grad")
     return g
 
 
-def _scan_args(what, x, delta, A, B, C, D, z, delta_bias, softplus, sharing, h_in, reset, lengths, record):
+def _scan_args(what, x, delta, A, B, C, D, z, delta_bias, sharing, h_in, reset, lengths, record):
+    """checked arguments: packed shape, device, shape of the state, sequences, addresses of A, D, delta_bias, h_in, reset, lengths, record"""
     if not isinstance(A, torch.Tensor) or A.dim() != 3:
         raise ValueError(f"{what}: A is not a [networks][states][channels] tensor")
     if not isinstance(B, torch.Tensor) or B.dim() != 5:
         raise ValueError(f"{what}: B is not a [agents][steps][batch][groups][states] tensor")
     N, G = A.shape[1], B.shape[3]
-    s, M = _ssm_shape(what, x, N, G, sharing)
-    P, S, NB, Ch = x.shape
-    for name, t in (("x", x), ("delta", delta), ("z", z)):
-        _expect_seq(what, name, t, x.shape, x.dtype, x.device)
-    for name, t in (("B", B), ("C", C)):
-        _expect_seq(what, name, t, (P, S, NB, G, N), x.dtype, x.device)
-    _expect(what, "A", A, (M, N, Ch), torch.float32, x.device)
-    for name, t in (("D", D), ("delta_bias", delta_bias)):
-        _expect(what, name, t, (M, Ch), torch.float32, x.device)
-    _expect(what, "h_in", h_in, (P, NB, N, Ch), torch.float32, x.device)
-    reset, lengths = _episode_flags(what, x, reset, lengths)
+    shape, M, dev = _ssm_shape(what, x, N, G, sharing)
+    P, S, NB, Ch = xshape = x.shape
+    dt, mshape, hshape = x.dtype, (P, S, NB, G, N), (P, NB, N, Ch)
+    seqs = (_seq(what, "x", x, xshape, dt, dev) + _seq(what, "delta", delta, xshape, dt, dev) + _seq(what, "B", B, mshape, dt, dev)
+            + _seq(what, "C", C, mshape, dt, dev) + _seq(what, "z", z, xshape, dt, dev))
+    if delta is None or C is None:
+        raise ValueError(f"{what}: delta and C are not optional")
+    rec = 0
     if record is not None:
-        n = check(lib.marlhip_ssm_scan_record_floats(ctypes.byref(s)), "ssm_scan_record_floats")
-        _expect(what, "record", record, (n,), torch.float32, x.device)
-    a = SsmScanArgs()
-    a.x, a.delta, a.B, a.C, a.z = _seq(x), _seq(delta), _seq(B), _seq(C), _seq(z)
-    a.A, a.D, a.delta_bias, a.softplus = _ptr(A), _ptr(D), _ptr(delta_bias), int(bool(softplus))
-    a.h_in, a.reset, a.lengths, a.record = _ptr(h_in), _ptr(reset), _ptr(lengths), _ptr(record)
-    return s, a, (P, NB, N, Ch)
+        rec = _dense(what, "record", record, (_ssm_size(lib.marlhip_ssm_scan_record_floats, "ssm_scan_record_floats", shape),), _F32, dev)
+    return (shape, dev, hshape, seqs, _dense(what, "A", A, (M, N, Ch), _F32, dev), _dense(what, "D", D, (M, Ch), _F32, dev),
+            _dense(what, "delta_bias", delta_bias, (M, Ch), _F32, dev), _dense(what, "h_in", h_in, hshape, _F32, dev),
+            *_episode_flags(what, x, reset, lengths, dev), rec)
 
 
 def ssm_scan_record(x, n_states):
     """the tensor ssm_scan leaves for ssm_scan_grad: the states its blocks of steps start from"""
-    s, _ = _ssm_shape("ssm_scan_record", x, n_states, 1, None)
-    n = check(lib.marlhip_ssm_scan_record_floats(ctypes.byref(s)), "ssm_scan_record_floats")
-    return torch.empty(n, dtype=torch.float32, device=x.device)
+    shape, _, _ = _ssm_shape("ssm_scan_record", x, int(n_states), 1, None)
+    return torch.empty(_ssm_size(lib.marlhip_ssm_scan_record_floats, "ssm_scan_record_floats", shape), dtype=_F32, device=x.device)
 
 
 def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=True, sharing=None, h_in=None, want_h=False, h_out=None, reset=None,
@@ -1514,18 +1528,19 @@ def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=True, 
     softplus=False takes dt = delta + delta_bias.  State f32 [P][B][N][C]: `h_in` (None: zeros), returned with want_h or written to `h_out`
     (`h_in` itself: updated in place).  `sharing`, `reset`, `lengths` as in ssm_conv.  `record` (ssm_scan_record): filled for ssm_scan_grad.
     -> y, or (y, h_out)"""
-    s, a, hshape = _scan_args("ssm_scan", x, delta, A, B, C, D, z, delta_bias, softplus, sharing, h_in, reset, lengths, record)
-    _expect("ssm_scan", "h_out", h_out, hshape, torch.float32, x.device)
+    shape, dev, hshape, seqs, pA, pD, pb, ph, rs, ln, rec = _scan_args("ssm_scan", x, delta, A, B, C, D, z, delta_bias, sharing, h_in, reset, lengths, record)
+    ho = _dense("ssm_scan", "h_out", h_out, hshape, _F32, dev)
     _in_place_or_apart("ssm_scan", "h_out", h_out, h_in)
-    _need_device("ssm_scan", x)
-    with _on_device(x):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if want_h and h_out is None:
-            h_out = torch.empty(hshape, dtype=torch.float32, device=x.device)
-        a.y, a.h_out = _ptr(y), _ptr(h_out)
-        n = check(lib.marlhip_ssm_scan_workspace_bytes(ctypes.byref(s)), "ssm_scan_workspace_bytes")
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        check(lib.marlhip_ssm_scan(ctypes.byref(s), ctypes.byref(a), _ptr(ws), n, _stream()), "ssm_scan")
+    _need_device("ssm_scan", x, dev)
+    n = _ssm_size(lib.marlhip_ssm_scan_workspace_bytes, "ssm_scan_workspace_bytes", shape)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if want_h and h_out is None:
+        h_out = torch.empty(hshape, dtype=_F32, device=x.device)
+        ho = h_out.data_ptr()
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device).data_ptr() if n else 0
+    args = _SCAN_PACK(*seqs, *_NO_SEQ, pA, pD, pb, 1 if softplus else 0, ph, rs, ln, y.data_ptr(), ho, rec, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    if _launch("ssm_scan", dev, lambda stream: lib.marlhip_ssm_scan(shape, args, ws, n, stream)) < 0:
+        check(-1, "ssm_scan")
     return (y, h_out) if want_h else y
 
 
@@ -1533,79 +1548,86 @@ def ssm_scan_grad(dy, x, delta, A, B, C, record, D=None, z=None, delta_bias=None
                   dh_out=None):
     """gradients of ssm_scan for the same arguments and the record it filled: dy [P][S][B][C] at y and (optional) dh_out [P][B][N][C] at h_out ->
     SsmScanGrad(x, delta, A, B, C, D, z, delta_bias, h_in); those of absent arguments are None"""
-    s, a, hshape = _scan_args("ssm_scan_grad", x, delta, A, B, C, D, z, delta_bias, softplus, sharing, h_in, reset, lengths, record)
+    what = "ssm_scan_grad"
+    shape, dev, hshape, seqs, pA, pD, pb, ph, rs, ln, rec = _scan_args(what, x, delta, A, B, C, D, z, delta_bias, sharing, h_in, reset, lengths, record)
     if record is None:
         raise ValueError("ssm_scan_grad: record is missing (ssm_scan fills it: record=ssm_scan_record(x, n_states))")
-    _expect_seq("ssm_scan_grad", "dy", dy, x.shape, x.dtype, x.device)
-    _expect("ssm_scan_grad", "dh_out", dh_out, hshape, torch.float32, x.device)
-    _need_device("ssm_scan_grad", x)
-    with _on_device(x):
-        def like(t, dtype=None):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    dys, dho = _seq(what, "dy", dy, x.shape, x.dtype, dev), _dense(what, "dh_out", dh_out, hshape, _F32, dev)
+    _need_device(what, x, dev)
+    n = _ssm_size(lib.marlhip_ssm_scan_grad_workspace_bytes, "ssm_scan_grad_workspace_bytes", shape)
 
-        g = SsmScanGrad(like(x), like(delta), like(A), like(B), like(C), like(D), like(z), like(delta_bias), like(h_in))
-        a.dy, a.dh_out = _seq(dy), _ptr(dh_out)
-        a.dx, a.ddelta, a.dB, a.dC, a.dz = _ptr(g.x), _ptr(g.delta), _ptr(g.B), _ptr(g.C), _ptr(g.z)
-        a.dA, a.dD, a.ddelta_bias, a.dh_in = _ptr(g.A), _ptr(g.D), _ptr(g.delta_bias), _ptr(g.h_in)
-        n = check(lib.marlhip_ssm_scan_grad_workspace_bytes(ctypes.byref(s)), "ssm_scan_grad_workspace_bytes")
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        check(lib.marlhip_ssm_scan_grad(ctypes.byref(s), ctypes.byref(a), _ptr(ws), n, _stream()), "ssm_scan_grad")
+    def like(t):
+        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+    g = SsmScanGrad(like(x), like(delta), like(A), like(B), like(C), like(D), like(z), like(delta_bias), like(h_in))
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    out = (0 if t is None else t.data_ptr() for t in (g.x, g.delta, g.B, g.C, g.z, g.A, g.D, g.delta_bias, g.h_in))
+    args = _SCAN_PACK(*seqs, *dys, pA, pD, pb, 1 if softplus else 0, ph, rs, ln, 0, 0, rec, dho, *out)
+    if _launch(what, dev, lambda stream: lib.marlhip_ssm_scan_grad(shape, args, ws.data_ptr(), n, stream)) < 0:
+        check(-1, what)
     return g
 
 
 # ---- global gradient norm and clip over many tensors (csrc/grad_norm.hip) ------------------------------------------------------------
 
 
-def _norm_tensors(what, tensors, out=None):
-    tensors = list(tensors)
-    out = tensors if out is None else list(out)
-    if len(out) != len(tensors):
-        raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} tensors")
-    table = (TensorStruct * max(len(tensors), 1))()
-    spans = []
-    for i, (t, o) in enumerate(zip(tensors, out)):
+def _norm_words(what, kind, tensors, dev):
+    """(addresses, element counts, type codes) of the tensors, each checked"""
+    try:
+        codes = [_SEQ_DTYPES[t.dtype] for t in tensors]
+        if all([t.is_contiguous() for t in tensors]) and all([t.get_device() == dev for t in tensors]):
+            return [t.data_ptr() for t in tensors], [t.numel() for t in tensors], codes
+    except (AttributeError, KeyError, TypeError):
+        pass
+    for i, t in enumerate(tensors):
         if not isinstance(t, torch.Tensor) or t.dtype not in _SEQ_DTYPES:
-            raise ValueError(f"{what}: tensor {i} is not a float32, bfloat16 or float16 tensor")
-        _expect(what, f"tensor {i}", t, t.shape, t.dtype, tensors[0].device)
-        if o is not t:
-            _expect(what, f"output {i}", o, t.shape, t.dtype, tensors[0].device)
-        n = t.numel()
-        table[i] = TensorStruct(t.data_ptr(), o.data_ptr(), n, _SEQ_DTYPES[t.dtype])
-        if n:
-            spans.append((o.data_ptr(), o.data_ptr() + n * o.element_size(), i))
-            if o.data_ptr() != t.data_ptr():
-                spans.append((t.data_ptr(), t.data_ptr() + n * t.element_size(), i))
-    spans.sort()
-    for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
-        if start < end:
-            raise ValueError(f"{what}: tensors {i} and {j} overlap (each gradient once)")
-    return tensors, table
+            raise ValueError(f"{what}: {kind} {i} is not a float32, bfloat16 or float16 tensor")
+        _expect(what, f"{kind} {i}", t, t.shape, t.dtype, dev)
 
 
-def _norm_call(what, fn, tensors, table, *args):
+def _norm_table(what, tensors, out=None):
+    """checked tensors as an array of marlhip_tensor (four 64-bit words each)"""
+    tensors = list(tensors)
     if not tensors:
         raise ValueError(f"{what}: no tensors")
-    _need_device(what, tensors[0])
-    with _on_device(tensors[0]):
-        norm = torch.empty(1, dtype=torch.float32, device=tensors[0].device)
-        n = check(lib.marlhip_grad_norm_workspace_bytes(table, len(tensors)), "grad_norm_workspace_bytes")
-        ws = torch.empty(n, dtype=torch.uint8, device=norm.device)
-        check(fn(table, len(tensors), *args, _ptr(norm), _ptr(ws), n, _stream()), what)
-    return norm
+    dev = tensors[0].get_device() if isinstance(tensors[0], torch.Tensor) else -1
+    ptr, n, code = _norm_words(what, "tensor", tensors, dev)
+    optr = ptr
+    if out is not None:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} tensors")
+        optr, on, ocode = _norm_words(what, "output", out, dev)
+        if on != n or ocode != code:
+            i = next(i for i in range(len(n)) if on[i] != n[i] or ocode[i] != code[i])
+            raise ValueError(f"{what}: output {i} is {out[i].dtype} of {on[i]} elements, expected {tensors[i].dtype} of {n[i]}")
+    words = array.array("Q", [w for quad in zip(ptr, optr, n, code) for w in quad])
+    return tensors[0], dev, len(tensors), words, words.buffer_info()[0]
 
 
 def grad_norm(tensors):
     """2-norm over all elements of many (contiguous) tensors, f32 [1] on their device: the squares are summed in 64 bits in a fixed order.
     f32, bf16 and f16 tensors may be mixed."""
-    tensors, table = _norm_tensors("grad_norm", tensors)
-    return _norm_call("grad_norm", lib.marlhip_grad_norm, tensors, table)
+    first, dev, count, words, table = _norm_table("grad_norm", tensors)
+    _need_device("grad_norm", first, dev)
+    nb = check(lib.marlhip_grad_norm_workspace_bytes(table, count), "grad_norm_workspace_bytes")
+    norm, ws = torch.empty(1, dtype=_F32, device=first.device), torch.empty(nb, dtype=torch.uint8, device=first.device)
+    check(_launch("grad_norm", dev, lambda stream: lib.marlhip_grad_norm(table, count, norm.data_ptr(), ws.data_ptr(), nb, stream)), "grad_norm")
+    return norm
 
 
 def clip_grad_norm(tensors, max_norm, out=None):
-    """clip by the global norm (nn.utils.clip_grad_norm_): every tensor times min(max_norm / (norm + 1e-6), 1), in place or into `out` (same
-    shapes and types) -> the norm before the clip, f32 [1].  Nothing is copied to the host; a norm that is not finite shows in the result."""
+    """clip by the global norm (nn.utils.clip_grad_norm_): every tensor times min(max_norm / (norm + 1e-6), 1), in place or into `out` (as many
+    elements of the same types, contiguous) -> the norm before the clip, f32 [1].  Each gradient once: tensors that overlap are refused.
+    Nothing is copied to the host; a norm that is not finite shows in the result."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm: max_norm {max_norm}")
-    tensors, table = _norm_tensors("clip_grad_norm", tensors, out)
-    return _norm_call("clip_grad_norm", lib.marlhip_clip_grad_norm, tensors, table, max_norm)
+    first, dev, count, words, table = _norm_table("clip_grad_norm", tensors, out)
+    if lib.marlhip_tensors_apart(table, count) < 0:
+        raise ValueError(f"clip_grad_norm: {_lib.last_error()}")
+    _need_device("clip_grad_norm", first, dev)
+    nb = check(lib.marlhip_grad_norm_workspace_bytes(table, count), "grad_norm_workspace_bytes")
+    norm, ws = torch.empty(1, dtype=_F32, device=first.device), torch.empty(nb, dtype=torch.uint8, device=first.device)
+    check(_launch("clip_grad_norm", dev, lambda stream: lib.marlhip_clip_grad_norm(table, count, max_norm, norm.data_ptr(), ws.data_ptr(), nb, stream)), "clip_grad_norm")
+    return norm

@@ -926,6 +926,8 @@ typedef struct marlhip_tensor {
     int64_t n;
     int32_t dtype;  /* 0 f32, 1 bf16, 2 f16 */
 } marlhip_tensor;
+/* <0 (with the pair in the error text) if two of the tensors, or one and another's destination, share memory */
+int marlhip_tensors_apart(const marlhip_tensor* tensors, int32_t count);
 int64_t marlhip_grad_norm_workspace_bytes(const marlhip_tensor* tensors, int32_t count);
 int marlhip_grad_norm(const marlhip_tensor* tensors, int32_t count, float* norm_out, void* workspace, int64_t workspace_bytes, void* stream);
 int marlhip_clip_grad_norm(const marlhip_tensor* tensors, int32_t count, float max_norm, float* norm_out, void* workspace,

@@ -781,6 +781,28 @@ def test_scan_refuses_sizes_and_states():
         scan_grad_call(v, h.ssm_scan_record(v["x"], 4))
 
 
+def test_packed_arguments_match_the_structs():
+    """hip.py packs the C structs itself: same sizes and fields as _lib.py's classes"""
+    import ctypes
+
+    from codebase_amd import _lib
+
+    assert len(h._SHAPE_PACK(*range(24))) == ctypes.sizeof(_lib.SsmShape)
+    conv = _lib.SsmConvArgs.from_buffer_copy(h._CONV_PACK(*range(1, 22)))
+    scan = _lib.SsmScanArgs.from_buffer_copy(h._SCAN_PACK(*range(1, 45)))
+    for struct, first in ((conv, 1), (scan, 1)):
+        k = first
+        for name, kind in struct._fields_:
+            v = getattr(struct, name)
+            if kind is _lib.SsmSeq:
+                assert (v.data, v.agent_stride, v.step_stride, v.row_stride) == (k, k + 1, k + 2, k + 3), name
+                k += 4
+            else:
+                assert v == k, name
+                k += 1
+    assert ctypes.sizeof(_lib.TensorStruct) == 32
+
+
 def test_c_entry_points_refuse_bad_shapes():
     import ctypes
 
@@ -848,5 +870,8 @@ def test_conv_refuses_states_and_the_cpu():
     with pytest.raises(h.MarlHipError, match="CPU"):
         conv_call(v)
     with pytest.raises(h.MarlHipError, match="9 taps"):
-        big = make_conv(2, 5, 3, 12, 9, device="cpu")
-        h.check(h.lib.marlhip_ssm_conv_grad_workspace_bytes(h._ssm_shape("conv", big["x"], 9, 1, None)[0]))
+        import ctypes
+
+        from codebase_amd._lib import SsmShape, check, lib
+
+        check(lib.marlhip_ssm_conv_grad_workspace_bytes(ctypes.byref(SsmShape(2, 5, 3, 12, 9, 1, 0, 0))))
