@@ -1,8 +1,9 @@
 // Global 2-norm over many tensors and the clip: marlhip_grad_norm, marlhip_clip_grad_norm.
 //
-// The tensors' pointers travel in the kernel's own arguments, up to NORM_ENTRIES a launch: no table has to be copied to the device, and a
-// captured graph holds them.  A first pass leaves one 64-bit sum of squares a workgroup, a second one adds them up in every workgroup (the
-// same order everywhere) and scales.  Bound by HBM: the gradients are read once or twice and written once.
+// The tensors' pointers travel in the kernel's own arguments, up to 160 a launch: no table has to be copied to the device, and a captured
+// graph holds them.  A first pass leaves one 64-bit sum of squares a workgroup, a second one adds them up in every workgroup (the same order
+// everywhere) and scales, in the opposite direction: what the first pass read last is still in the caches.  Bound by HBM: the gradients are
+// read twice, less what the caches keep, and written once.
 #include <algorithm>
 #include <vector>
 
@@ -12,8 +13,9 @@ using namespace marl;
 
 namespace {
 
-constexpr int NORM_ENTRIES = 160;
 constexpr int64_t NORM_PIECE = 1ll << 30;  // elements of an entry (larger tensors take several)
+constexpr int64_t NORM_WGS = 4096;         // workgroups of a pass, about
+constexpr int FEW = 16, MANY = 160;        // entries of a launch (the small table saves the host's copy of the large one)
 
 struct NormEntry {
     const void* p;
@@ -21,32 +23,70 @@ struct NormEntry {
     uint32_t n;
     uint32_t first;  // first workgroup of the launch that works on it, type in the top two bits
 };
+template <int E>
 struct NormTable {
-    NormEntry e[NORM_ENTRIES];
+    NormEntry e[E];
     int count;
     uint32_t chunk;    // elements a workgroup takes
     int part0, parts;  // first partial sum of the launch; all of the call's
     float max_norm;
+    int stream;  // stores past the caches
 };
-static_assert(sizeof(NormTable) <= 4000, "kernel arguments");
+static_assert(sizeof(NormTable<MANY>) <= 4000, "kernel arguments");
 
+template <int W>
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+    v = 0.0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) v += red[w];
     __syncthreads();
     return v;
 }
 
-template <class T, int V>
-struct alignas(V * sizeof(T)) NVec {
-    T v[V];
+__device__ __forceinline__ float clip_coef(float max_norm, float norm) {
+    const float ratio = max_norm / (norm + 1e-6f);
+    return ratio > 1.f ? 1.f : ratio;  // NaN stays NaN
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <class T>
+struct Pack {  // 16 bytes of elements
+    static constexpr int V = 16 / sizeof(T);
+    u32x4 w;
+    __device__ __forceinline__ T get(int j) const {
+        const uint32_t x = w[sizeof(T) == 4 ? j : j / 2];
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, x);
+        else return __builtin_bit_cast(T, (unsigned short)(x >> (j % 2 * 16)));
+    }
+    __device__ __forceinline__ void scale(float coef) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = __builtin_bit_cast(uint32_t, get(i) * coef);
+            } else {
+                const T lo = static_cast<T>(static_cast<float>(get(2 * i)) * coef), hi = static_cast<T>(static_cast<float>(get(2 * i + 1)) * coef);
+                w[i] = (uint32_t)__builtin_bit_cast(unsigned short, lo) | ((uint32_t)__builtin_bit_cast(unsigned short, hi) << 16);
+            }
+        }
+    }
+    __device__ __forceinline__ double squares() const {
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const double g = static_cast<float>(get(j));
+            s = fma(g, g, s);
+        }
+        return s;
+    }
 };
 
 // the entry of this workgroup, and its elements [i0, i1)
-__device__ __forceinline__ const NormEntry& find_entry(const NormTable& t, uint32_t blk, uint32_t& i0, uint32_t& i1) {
+template <int E>
+__device__ __forceinline__ const NormEntry& find_entry(const NormTable<E>& t, uint32_t blk, uint32_t& i0, uint32_t& i1) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {  // the last entry whose first workgroup is not behind this one
         const int mid = (lo + hi + 1) >> 1;
@@ -59,62 +99,81 @@ __device__ __forceinline__ const NormEntry& find_entry(const NormTable& t, uint3
     return e;
 }
 
+constexpr int U = 4;  // 16-byte requests of a thread in flight
+
 template <class T>
 __device__ __forceinline__ double square_sum(const T* p, uint32_t i0, uint32_t i1) {
-    constexpr int V = 16 / sizeof(T);
-    double s = 0.0;
+    constexpr int V = Pack<T>::V;
+    double s[U] = {};
     uint32_t i = i0;
     if ((uintptr_t)p % 16 == 0) {
+        const Pack<T>* v = reinterpret_cast<const Pack<T>*>(p + i0);
         const uint32_t nv = (i1 - i0) / V;
-        for (uint32_t k = threadIdx.x; k < nv; k += 256) {
-            const NVec<T, V> q = *reinterpret_cast<const NVec<T, V>*>(p + i0 + k * V);
+        uint32_t k = threadIdx.x;
+        for (; k + (U - 1) * 256 < nv; k += U * 256) {
+            Pack<T> q[U];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const double g = static_cast<float>(q.v[j]);
-                s = fma(g, g, s);
-            }
+            for (int u = 0; u < U; ++u) q[u] = v[k + u * 256];
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] += q[u].squares();
         }
+        for (; k < nv; k += 256) s[0] += v[k].squares();
         i = i0 + nv * V;
     }
     for (uint32_t k = i + threadIdx.x; k < i1; k += 256) {
         const double g = static_cast<float>(p[k]);
-        s = fma(g, g, s);
+        s[0] = fma(g, g, s[0]);
     }
-    return s;
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <class T>
+template <class T, bool STREAM>
 __device__ __forceinline__ void scale_all(const T* p, T* o, float coef, uint32_t i0, uint32_t i1) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = Pack<T>::V;
     uint32_t i = i0;
     if (((uintptr_t)p | (uintptr_t)o) % 16 == 0) {
+        const Pack<T>* v = reinterpret_cast<const Pack<T>*>(p + i0);
+        u32x4* w = reinterpret_cast<u32x4*>(o + i0);
         const uint32_t nv = (i1 - i0) / V;
-        for (uint32_t k = threadIdx.x; k < nv; k += 256) {
-            NVec<T, V> q = *reinterpret_cast<const NVec<T, V>*>(p + i0 + k * V);
+        uint32_t k = threadIdx.x;
+        for (; k + (U - 1) * 256 < nv; k += U * 256) {
+            Pack<T> q[U];
 #pragma unroll
-            for (int j = 0; j < V; ++j) q.v[j] = static_cast<T>(static_cast<float>(q.v[j]) * coef);
-            *reinterpret_cast<NVec<T, V>*>(o + i0 + k * V) = q;
+            for (int u = 0; u < U; ++u) q[u] = v[k + u * 256];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                q[u].scale(coef);
+                if (STREAM) __builtin_nontemporal_store(q[u].w, w + k + u * 256);
+                else w[k + u * 256] = q[u].w;
+            }
+        }
+        for (; k < nv; k += 256) {
+            Pack<T> q = v[k];
+            q.scale(coef);
+            w[k] = q.w;
         }
         i = i0 + nv * V;
     }
     for (uint32_t k = i + threadIdx.x; k < i1; k += 256) o[k] = static_cast<T>(static_cast<float>(p[k]) * coef);
 }
 
-__global__ __launch_bounds__(256) void grad_square_kernel(NormTable t, double* __restrict__ part) {
+template <int E>
+__global__ __launch_bounds__(256) void grad_square_kernel(NormTable<E> t, double* __restrict__ part) {
     __shared__ double red[4];
     uint32_t i0, i1;
     const NormEntry& e = find_entry(t, blockIdx.x, i0, i1);
     const int dt = e.first >> 30;
     const double s = dt == 0 ? square_sum(static_cast<const float*>(e.p), i0, i1)
                              : (dt == 1 ? square_sum(static_cast<const __bf16*>(e.p), i0, i1) : square_sum(static_cast<const _Float16*>(e.p), i0, i1));
-    const double sum = block_sum(s, red);
+    const double sum = block_sum<4>(s, red);
     if (threadIdx.x == 0) part[t.part0 + blockIdx.x] = sum;
 }
 
 __device__ __forceinline__ float total_norm(const double* part, int parts, double* red) {
     double s = 0.0;
+#pragma unroll 4
     for (int k = threadIdx.x; k < parts; k += 256) s += part[k];
-    return (float)sqrt(block_sum(s, red));
+    return (float)sqrt(block_sum<4>(s, red));
 }
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict__ part, int parts, float* __restrict__ norm_out) {
@@ -123,36 +182,46 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict
     if (threadIdx.x == 0) norm_out[0] = norm;
 }
 
-__global__ __launch_bounds__(256) void grad_clip_kernel(NormTable t, const double* __restrict__ part, float* __restrict__ norm_out) {
+template <bool STREAM>
+__device__ __forceinline__ void scale_entry(const NormEntry& e, float coef, uint32_t i0, uint32_t i1) {
+    const int dt = e.first >> 30;
+    if (dt == 0) scale_all<float, STREAM>(static_cast<const float*>(e.p), static_cast<float*>(e.o), coef, i0, i1);
+    else if (dt == 1) scale_all<__bf16, STREAM>(static_cast<const __bf16*>(e.p), static_cast<__bf16*>(e.o), coef, i0, i1);
+    else scale_all<_Float16, STREAM>(static_cast<const _Float16*>(e.p), static_cast<_Float16*>(e.o), coef, i0, i1);
+}
+
+template <int E>
+__global__ __launch_bounds__(256) void grad_clip_kernel(NormTable<E> t, const double* __restrict__ part, float* __restrict__ norm_out) {
     __shared__ double red[4];
     const float norm = total_norm(part, t.parts, red);
     if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
-    const float ratio = t.max_norm / (norm + 1e-6f), coef = ratio > 1.f ? 1.f : ratio;  // NaN stays NaN
+    const float coef = clip_coef(t.max_norm, norm);
     uint32_t i0, i1;
     const NormEntry& e = find_entry(t, blockIdx.x, i0, i1);
-    const int dt = e.first >> 30;
-    if (dt == 0) scale_all(static_cast<const float*>(e.p), static_cast<float*>(e.o), coef, i0, i1);
-    else if (dt == 1) scale_all(static_cast<const __bf16*>(e.p), static_cast<__bf16*>(e.o), coef, i0, i1);
-    else scale_all(static_cast<const _Float16*>(e.p), static_cast<_Float16*>(e.o), coef, i0, i1);
+    if (t.stream) scale_entry<true>(e, coef, i0, i1);
+    else scale_entry<false>(e, coef, i0, i1);
 }
 
 struct NormPlan {
     int64_t chunk, parts;
+    bool stream;  // more bytes than half of the last-level cache: what is written does not push out what is still to be read
 };
 
 int norm_plan(const marlhip_tensor* t, int32_t count, NormPlan& plan, bool clip) {
     MARL_REQUIRE(count >= 0 && (count == 0 || t != nullptr), "grad_norm: %d tensors", count);
-    int64_t total = 0;
+    int64_t total = 0, bytes = 0;
     for (int i = 0; i < count; ++i) {
         MARL_REQUIRE(t[i].n >= 0 && t[i].n < (1ll << 40) && (t[i].n == 0 || t[i].data != nullptr), "grad_norm: tensor %d", i);
         MARL_REQUIRE(t[i].dtype >= 0 && t[i].dtype <= 2, "grad_norm: tensor %d: dtype %d (0 f32, 1 bf16, 2 f16)", i, t[i].dtype);
         const int e = t[i].dtype == 0 ? 4 : 2;
         MARL_REQUIRE((uintptr_t)t[i].data % e == 0 && (!clip || (uintptr_t)t[i].out % e == 0), "grad_norm: tensor %d is not aligned to its type", i);
         total += t[i].n;
+        bytes += t[i].n * e;
     }
-    // about 2048 workgroups: enough to fill the chip, few enough sums for every one of them to add up
-    const int64_t c = (total / 2048 + 4095) / 4096 * 4096;
+    // about 4096 workgroups: enough to fill the chip evenly (2048 took 15 % longer on 57 M elements), few enough sums for every one to add up
+    const int64_t c = (total / NORM_WGS + 4095) / 4096 * 4096;
     plan.chunk = c < 4096 ? 4096 : c;
+    plan.stream = bytes > (1ll << 27);
     plan.parts = 0;
     for (int i = 0; i < count; ++i)
         for (int64_t o = 0; o < t[i].n; o += NORM_PIECE) {
@@ -163,15 +232,16 @@ int norm_plan(const marlhip_tensor* t, int32_t count, NormPlan& plan, bool clip)
     return 0;
 }
 
-// launch(table, workgroups) for every NORM_ENTRIES pieces
-template <class F>
-int norm_tables(const marlhip_tensor* t, int32_t count, const NormPlan& plan, float max_norm, F launch) {
-    NormTable tab;
+// launch(table, workgroups) for every E pieces, from the last tensor to the first if reverse
+template <int E, class F>
+int norm_tables(const marlhip_tensor* t, int32_t count, const NormPlan& plan, float max_norm, bool reverse, F launch) {
+    NormTable<E> tab;
     tab.count = 0;
     tab.chunk = (uint32_t)plan.chunk;
     tab.part0 = 0;
     tab.parts = (int)plan.parts;
     tab.max_norm = max_norm;
+    tab.stream = plan.stream;
     uint32_t blocks = 0;
     auto flush = [&]() {
         if (tab.count == 0) return 0;
@@ -181,10 +251,10 @@ int norm_tables(const marlhip_tensor* t, int32_t count, const NormPlan& plan, fl
         blocks = 0;
         return rc;
     };
-    for (int i = 0; i < count; ++i) {
-        const int es = t[i].dtype == 0 ? 4 : 2;
+    for (int j = 0; j < count; ++j) {
+        const int i = reverse ? count - 1 - j : j, es = t[i].dtype == 0 ? 4 : 2;
         for (int64_t o = 0; o < t[i].n; o += NORM_PIECE) {
-            if (tab.count == NORM_ENTRIES && flush() != 0) return -2;
+            if (tab.count == E && flush() != 0) return -2;
             const int64_t n = t[i].n - o < NORM_PIECE ? t[i].n - o : NORM_PIECE;
             NormEntry& e = tab.e[tab.count++];
             e.p = static_cast<const char*>(t[i].data) + o * es;
@@ -197,10 +267,21 @@ int norm_tables(const marlhip_tensor* t, int32_t count, const NormPlan& plan, fl
     return flush();
 }
 
+template <int E>
 int square_pass(const marlhip_tensor* t, int32_t count, const NormPlan& plan, double* part, hipStream_t st) {
-    return norm_tables(t, count, plan, 0.f, [&](const NormTable& tab, uint32_t blocks) {
-        hipLaunchKernelGGL(grad_square_kernel, dim3(blocks), dim3(256), 0, st, tab, part);
+    return norm_tables<E>(t, count, plan, 0.f, false, [&](const NormTable<E>& tab, uint32_t blocks) {
+        hipLaunchKernelGGL(grad_square_kernel<E>, dim3(blocks), dim3(256), 0, st, tab, part);
         MARL_CHECK_LAUNCH("grad_square_kernel");
+        return 0;
+    });
+}
+
+template <int E>
+int clip_passes(const marlhip_tensor* t, int32_t count, const NormPlan& plan, float max_norm, double* part, float* norm_out, hipStream_t st) {
+    if (square_pass<E>(t, count, plan, part, st) != 0) return -2;
+    return norm_tables<E>(t, count, plan, max_norm, true, [&](const NormTable<E>& tab, uint32_t blocks) {
+        hipLaunchKernelGGL(grad_clip_kernel<E>, dim3(blocks), dim3(256), 0, st, tab, part, norm_out);
+        MARL_CHECK_LAUNCH("grad_clip_kernel");
         return 0;
     });
 }
@@ -252,7 +333,7 @@ extern "C" int marlhip_grad_norm(const marlhip_tensor* tensors, int32_t count, f
     MARL_REQUIRE(norm_out != nullptr, "grad_norm: NULL pointer");
     double* part = static_cast<double*>(workspace);
     hipStream_t st = (hipStream_t)stream;
-    if (square_pass(tensors, count, plan, part, st) != 0) return -2;
+    if ((count <= FEW ? square_pass<FEW>(tensors, count, plan, part, st) : square_pass<MANY>(tensors, count, plan, part, st)) != 0) return -2;
     hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, st, part, (int)plan.parts, norm_out);
     MARL_CHECK_LAUNCH("grad_norm_kernel");
     return 0;
@@ -271,10 +352,6 @@ extern "C" int marlhip_clip_grad_norm(const marlhip_tensor* tensors, int32_t cou
         MARL_CHECK_LAUNCH("grad_norm_kernel");
         return 0;
     }
-    if (square_pass(tensors, count, plan, part, st) != 0) return -2;
-    return norm_tables(tensors, count, plan, max_norm, [&](const NormTable& tab, uint32_t blocks) {
-        hipLaunchKernelGGL(grad_clip_kernel, dim3(blocks), dim3(256), 0, st, tab, part, norm_out);
-        MARL_CHECK_LAUNCH("grad_clip_kernel");
-        return 0;
-    });
+    return count <= FEW ? clip_passes<FEW>(tensors, count, plan, max_norm, part, norm_out, st)
+                        : clip_passes<MANY>(tensors, count, plan, max_norm, part, norm_out, st);
 }

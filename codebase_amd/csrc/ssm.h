@@ -37,15 +37,16 @@ constexpr int OOB = (int)0x80000000;   // an offset behind any row
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* base, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
 }
+// (soff: a uniform offset that the bound does not count)
 template <class T>
-__device__ __forceinline__ float row_load(const T* base, int bytes, int voff) {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(row_rsrc(base, bytes), voff, 0, 0));
-    else return up(__builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(row_rsrc(base, bytes), voff, 0, 0)));
+__device__ __forceinline__ float row_load(const T* base, int bytes, int voff, int soff = 0) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(row_rsrc(base, bytes), voff, soff, 0));
+    else return up(__builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(row_rsrc(base, bytes), voff, soff, 0)));
 }
 template <class T>
-__device__ __forceinline__ void row_store(float v, T* base, int bytes, int voff) {
-    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), row_rsrc(base, bytes), voff, 0, 0);
-    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, down<T>(v)), row_rsrc(base, bytes), voff, 0, 0);
+__device__ __forceinline__ void row_store(float v, T* base, int bytes, int voff, int soff = 0) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), row_rsrc(base, bytes), voff, soff, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, down<T>(v)), row_rsrc(base, bytes), voff, soff, 0);
 }
 
 struct SsmDims {

@@ -16,6 +16,7 @@ namespace {
 
 constexpr int K = 8;     // steps of a block: between two recorded states
 constexpr int WMAX = 8;  // waves of a backward workgroup
+constexpr int STEP_WAVES = 8192;  // waves of an acting step
 
 struct ScanArgs {
     SsmDims d;
@@ -62,7 +63,7 @@ template <int NL, int NS>
 __device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<NL, NS>& q, const float* p, float scale, float (&r)[NL]) {
     const int off = q.state_off(a), bytes = p != nullptr ? ROW_MAX : 0;
 #pragma unroll
-    for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first + (int64_t)n * a.d.C, bytes, off | q.no_state(a, n));
+    for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first, bytes, off | q.no_state(a, n), n * a.d.C * 4);
 #pragma unroll
     for (int n = 0; n < NL; ++n) r[n] *= scale;
 }
@@ -70,7 +71,7 @@ template <int NL, int NS>
 __device__ __forceinline__ void store_state(const ScanArgs& a, const Lane<NL, NS>& q, float* p, const float (&r)[NL]) {
     const int off = q.state_off(a);
 #pragma unroll
-    for (int n = 0; n < NL; ++n) row_store(r[n], p + q.first + (int64_t)n * a.d.C, ROW_MAX, off | q.no_state(a, n));
+    for (int n = 0; n < NL; ++n) row_store(r[n], p + q.first, ROW_MAX, off | q.no_state(a, n), n * a.d.C * 4);
 }
 
 // value of group i of a register that holds one value a group, in every group
@@ -317,6 +318,79 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     yp = static_cast<T*>(a.y) + ((int64_t)p * a.d.S * a.d.B + b) * C + q.first;
     for (int t = end > first ? end : first; t < last; ++t) row_store(0.f, yp + t * yst, ROW_MAX, q.g == 0 ? q.chan_off(sizeof(T)) : OOB);
     if (a.h_out != nullptr && ch == a.nchunk - 1) store_state(a, q, a.h_out + (int64_t)row * N * C, h);
+}
+
+// One step a row (acting).  All there is to do is to read a row's state, to move it on and to write it back: a lane keeps one channel with all
+// its states, so that nothing crosses lanes, a wave takes rows b = slot, slot + slots, .. of one agent with its decay rates in registers, and the
+// next row is requested before the current one is worked on.
+template <class T, int NP>
+__global__ __launch_bounds__(256) void ssm_scan_step_kernel(ScanArgs a) {
+    __shared__ float lds[4][2][NP];
+    const int wv = uni(threadIdx.x >> 6);
+    const int item = blockIdx.x * 4 + wv;
+    if (item >= a.items) return;
+    const int ncb = a.d.G * a.nblk, ps = uni(item / ncb), cb = item - ps * ncb, p = uni(ps / a.slots), slot = ps - p * a.slots;
+    const Lane<NP, 1> q(a, cb, threadIdx.x & 63);
+    const int N = a.d.N, C = a.d.C, NB = a.d.B, net = a.d.net[p], lane = q.lane;
+    const int ct = q.chan_off(sizeof(T)), cf = q.chan_off(4);
+    float A[NP], h[NP], nh[NP];
+    Raw<T> x, d, z, m;
+    int rs, ln;
+    const bool gated = a.z.data != nullptr;
+    // lanes 0 .. N-1 fetch B, lanes NP .. NP+N-1 (of 2 NP <= 64) C
+    const bool isC = lane >= NP;
+    const int n_of = isC ? lane - NP : lane;
+    const bool fetch = n_of < N;
+    const int hbytes = a.h_in != nullptr ? ROW_MAX : 0;
+    auto request = [&](int b) __attribute__((always_inline)) {
+        x.load(seq_at<T>(a.x, p, b) + q.first, ct);
+        d.load(seq_at<T>(a.delta, p, b) + q.first, ct);
+        if (gated) z.load(seq_at<T>(a.z, p, b) + q.first, ct);
+        const T* mp = (isC ? seq_at<T>(a.Cm, p, b) : seq_at<T>(a.Bm, p, b)) + q.grp * N + (fetch ? n_of : 0);
+        m.v = *reinterpret_cast<const decltype(m.v)*>(mp);
+        rs = a.reset != nullptr ? a.reset[b] : 0;
+        ln = a.lengths != nullptr ? a.lengths[b] : 1;
+        const float* hp = a.h_in + ((int64_t)p * NB + b) * N * C + q.first;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) nh[n] = row_load(hp, hbytes, n < N ? cf : OOB, n * C * 4);
+    };
+    request(slot);
+    const float* Ap = a.A + (int64_t)net * N * C + q.first;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) A[n] = row_load(Ap, ROW_MAX, n < N ? cf : OOB, n * C * 4);
+    const float D = row_load(a.D + (int64_t)net * C + q.first, a.D != nullptr ? ROW_MAX : 0, cf);
+    const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, cf);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) A[n] *= LOG2E;
+    float* lm = lds[wv][0];
+    for (int b = slot; b < NB; b += a.slots) {
+        const bool fresh = uni(rs) != 0, live = uni(ln) > 0;
+        wave_lds_sync();
+        if (lane < 2 * NP) lm[lane] = fetch ? m.get() : 0.f;
+        wave_lds_sync();
+        const float xv = x.get(), dv = d.get(), zv = gated ? z.get() : 0.f;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) h[n] = fresh && live ? 0.f : nh[n];
+        if (b + a.slots < NB) request(b + a.slots);
+        float y = 0.f;
+        if (live) {
+            const float dt = step_size(a, dv, bias), u = dt * xv;
+            y = D * xv;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                h[n] = fmaf(exp2_fast(dt * A[n]), h[n], u * lm[n]);
+                y = fmaf(h[n], lm[NP + n], y);
+            }
+            if (gated) y *= zv * sigmoid(zv);
+        }
+        const int64_t row = (int64_t)p * NB + b;
+        row_store(y, static_cast<T*>(a.y) + row * C + q.first, ROW_MAX, ct);
+        if (a.h_out != nullptr) {
+            float* hp = a.h_out + row * N * C + q.first;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) row_store(h[n], hp, ROW_MAX, n < N ? cf : OOB, n * C * 4);
+        }
+    }
 }
 
 // Joins the chunks of a sequence: carry[j] (what chunk j contributes) becomes what chunk j starts from.  A chunk multiplies what it is given by
@@ -796,6 +870,26 @@ int join(const ScanArgs& a, const float* start, int reverse, hipStream_t st) {
     return 0;
 }
 
+int scan_step(const marlhip_ssm_shape* s, ScanArgs a, hipStream_t st) {
+    a.nblk = (s->channels / s->groups + 63) / 64;
+    const int64_t per = (int64_t)s->n_agents * s->groups * a.nblk;  // waves that one row of every agent takes
+    const int64_t slots = STEP_WAVES / per;
+    a.slots = (int)(slots < 1 ? 1 : (slots < s->batch ? slots : s->batch));
+    a.items = (int)(per * a.slots);
+    const dim3 grid((unsigned)((a.items + 3) / 4));
+    auto by_state = [&](auto t) {
+        using T = decltype(t);
+        if (s->state <= 8) hipLaunchKernelGGL((ssm_scan_step_kernel<T, 8>), grid, dim3(256), 0, st, a);
+        else if (s->state <= 16) hipLaunchKernelGGL((ssm_scan_step_kernel<T, 16>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ssm_scan_step_kernel<T, 32>), grid, dim3(256), 0, st, a);
+    };
+    if (s->dtype == 0) by_state(float{});
+    else if (s->dtype == 1) by_state(__bf16{});
+    else by_state(_Float16{});
+    MARL_CHECK_LAUNCH("ssm_scan_step_kernel");
+    return 0;
+}
+
 }  // namespace
 
 extern "C" int64_t marlhip_ssm_scan_record_floats(const marlhip_ssm_shape* s) {
@@ -820,6 +914,7 @@ extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_sc
                  (long long)workspace_bytes);
     if (s->batch == 0) return 0;
     ScanArgs a = scan_args(s, q, pl);
+    if (s->steps == 1 && a.record == nullptr) return scan_step(s, a, (hipStream_t)stream);
     a.items = (int)scan_items(s, pl);
     const dim3 grid((unsigned)((a.items + 3) / 4));
     hipStream_t st = (hipStream_t)stream;

@@ -3,6 +3,7 @@ current torch stream, nothing copied to the host.  torch is plumbing here (devic
 streams); every computation below happens in the HIP library."""
 import array
 import ctypes
+import operator
 import struct
 from collections import namedtuple
 from dataclasses import dataclass
@@ -1571,12 +1572,16 @@ def ssm_scan_grad(dy, x, delta, A, B, C, record, D=None, z=None, delta_bias=None
 # ---- global gradient norm and clip over many tensors (csrc/grad_norm.hip) ------------------------------------------------------------
 
 
+_DTYPE_OF = operator.attrgetter("dtype")
+
+
 def _norm_words(what, kind, tensors, dev):
-    """(addresses, element counts, type codes) of the tensors, each checked"""
+    """(addresses, element counts, type codes) of the tensors, each checked (map over the methods: a list may hold hundreds)"""
+    T = torch.Tensor
     try:
-        codes = [_SEQ_DTYPES[t.dtype] for t in tensors]
-        if all([t.is_contiguous() for t in tensors]) and all([t.get_device() == dev for t in tensors]):
-            return [t.data_ptr() for t in tensors], [t.numel() for t in tensors], codes
+        codes = list(map(_SEQ_DTYPES.__getitem__, map(_DTYPE_OF, tensors)))
+        if all(map(T.is_contiguous, tensors)) and set(map(T.get_device, tensors)) == {dev}:
+            return list(map(T.data_ptr, tensors)), list(map(T.numel, tensors)), codes
     except (AttributeError, KeyError, TypeError):
         pass
     for i, t in enumerate(tensors):
@@ -1601,7 +1606,9 @@ def _norm_table(what, tensors, out=None):
         if on != n or ocode != code:
             i = next(i for i in range(len(n)) if on[i] != n[i] or ocode[i] != code[i])
             raise ValueError(f"{what}: output {i} is {out[i].dtype} of {on[i]} elements, expected {tensors[i].dtype} of {n[i]}")
-    words = array.array("Q", [w for quad in zip(ptr, optr, n, code) for w in quad])
+    words = array.array("Q", bytes(32 * len(n)))
+    for k, column in enumerate((ptr, optr, n, code)):
+        words[k::4] = array.array("Q", column)
     return tensors[0], dev, len(tensors), words, words.buffer_info()[0]
 
 
