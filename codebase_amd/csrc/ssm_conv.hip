@@ -21,6 +21,8 @@ struct ConvArgs {
     int W, silu, chunk, nchunk, slots;
 };
 
+constexpr int U = 4;  // steps requested together
+
 template <class T, int V>
 struct alignas(V * sizeof(T)) Vec {
     T v[V];
@@ -28,6 +30,11 @@ struct alignas(V * sizeof(T)) Vec {
 template <class T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float (&r)[V]) {
     const Vec<T, V> q = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = up(q.v[i]);
+}
+template <class T, int V>
+__device__ __forceinline__ void widen(const Vec<T, V>& q, float (&r)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) r[i] = up(q.v[i]);
 }
@@ -110,31 +117,40 @@ __global__ __launch_bounds__(256) void ssm_conv_fwd_kernel(ConvArgs a) {
     }
     T* yp = static_cast<T*>(a.y) + ((int64_t)p * a.d.S * a.d.B + b) * a.d.C + c;
     const int64_t yst = (int64_t)a.d.B * a.d.C;
-    for (int t = t0; t < t1; ++t) {
-        float y[V];
-        if (t < len) {
-            load_vec<T, V>(xp + t * a.x.st, win[0]);
-            if (RESET && a.reset[(int64_t)t * a.d.B + b] != 0) start = t;
+    for (int t = t0; t < t1; t += U) {
+        Vec<T, V> raw[U];
+        uint8_t fresh[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {  // U steps requested together; those behind the end are there, but not used
+            const int64_t tu = t + u < t1 ? t + u : t1 - 1;
+            raw[u] = *reinterpret_cast<const Vec<T, V>*>(xp + tu * a.x.st);
+            fresh[u] = RESET ? a.reset[tu * a.d.B + b] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (t + u >= t1) break;
+            float y[V];
+            widen<T, V>(raw[u], win[0]);
+            if (RESET && fresh[u] != 0) start = t + u;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float s = bias[e];
 #pragma unroll
                 for (int j = 0; j < WM; ++j)
                     if (!RESET || j == 0) s = fmaf(w[j][e], win[j][e], s);
-                    else s = t - j >= start ? fmaf(w[j][e], win[j][e], s) : s;
-                y[e] = a.silu ? s * sigmoid(s) : s;
+                    else s = t + u - j >= start ? fmaf(w[j][e], win[j][e], s) : s;
+                y[e] = t + u < len ? (a.silu ? s * sigmoid(s) : s) : 0.f;
             }
 #pragma unroll
             for (int j = WM - 1; j > 0; --j)
 #pragma unroll
                 for (int e = 0; e < V; ++e) win[j][e] = win[j - 1][e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = 0.f;
+            store_vec<T, V>(yp + (t + u) * yst, y);
         }
-        store_vec<T, V>(yp + t * yst, y);
     }
-    if (a.nchunk == 1 && a.state_out != nullptr) window_out<T, V, WM>(a, xp, p, b, c, len);
+    // the stretch with the row's last step leaves the window; updated in place it has to wait for the first stretch's reads (ssm_conv_window_kernel)
+    if (a.state_out != nullptr && (a.nchunk == 1 || a.state_out != a.state) && t0 == (len > 0 ? (len - 1) / a.chunk * a.chunk : 0))
+        window_out<T, V, WM>(a, xp, p, b, c, len);
 }
 
 template <class T, int V, int WM>
@@ -184,76 +200,93 @@ __global__ __launch_bounds__(256) void ssm_conv_bwd_kernel(ConvArgs a, int tile)
         for (int j = 0; j < WM; ++j)
 #pragma unroll
             for (int e = 0; e < V; ++e) de[j][e] = 0.f;
-        for (int t = t0; t < t1 + WM - 1; ++t) {
-            if (t < len && t < t1 + a.W - 1) {
-                float g[V];
-                load_vec<T, V>(xp + t * a.x.st, win[0]);
-                load_vec<T, V>(gp + t * a.dy.st, g);
-                if (RESET && a.reset[(int64_t)t * a.d.B + b] != 0) start = t;
+        const int tl = len < t1 + a.W - 1 ? len : t1 + a.W - 1;  // steps from tl on give nothing to this stretch
+        for (int tb = t0; tb < t1 + WM - 1; tb += U) {
+            Vec<T, V> rx[U], rg[U];
+            uint8_t fresh[U];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float s = bias[e], xw[WM];
-#pragma unroll
-                    for (int j = 0; j < WM; ++j) {
-                        xw[j] = !RESET || t - j >= start ? win[j][e] : 0.f;
-                        s = fmaf(w[j][e], xw[j], s);
-                    }
-                    if (a.silu) {
-                        const float sg = sigmoid(s);
-                        g[e] *= sg * fmaf(s, 1.f - sg, 1.f);
-                    }
-#pragma unroll
-                    for (int j = 0; j < WM; ++j)
-                        if (!RESET || t - j >= start) de[j][e] = fmaf(w[j][e], g[e], de[j][e]);
-                    if (t < t1) {
-                        db[e] += g[e];
-#pragma unroll
-                        for (int j = 0; j < WM; ++j) dw[j][e] = fmaf(xw[j], g[e], dw[j][e]);
-                    }
+            for (int u = 0; u < U; ++u) {
+                const int64_t tu = tb + u < a.d.S ? tb + u : a.d.S - 1;
+                if (tb < tl) {
+                    rx[u] = *reinterpret_cast<const Vec<T, V>*>(xp + tu * a.x.st);
+                    rg[u] = *reinterpret_cast<const Vec<T, V>*>(gp + tu * a.dy.st);
+                    fresh[u] = RESET ? a.reset[tu * a.d.B + b] : 0;
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) win[0][e] = 0.f;
-            }
-            const int q = t - (WM - 1);  // this input has met its last step
-            if ((q >= t0 || (t0 == 0 && q >= -(a.W - 1))) && q < t1) {
-                const int k = q - (len - (a.W - 1));  // its place in the window after the last step
-                if (a.dstate_out != nullptr && k >= 0 && k < a.W - 1 && q >= start) {
-                    float r[V];
-                    load_vec<T, V>(static_cast<const T*>(a.dstate_out) + (row * (a.W - 1) + k) * a.d.C + c, r);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) de[WM - 1][e] += r[e];
-                }
-                if (q >= 0) store_vec<T, V>(dxp + q * yst, de[WM - 1]);
-                else if (a.dstate != nullptr) store_vec<T, V>(static_cast<T*>(a.dstate) + (row * (a.W - 1) + a.W - 1 + q) * a.d.C + c, de[WM - 1]);
             }
 #pragma unroll
-            for (int j = WM - 1; j > 0; --j)
+            for (int u = 0; u < U; ++u) {
+                const int t = tb + u;
+                if (t >= t1 + WM - 1) break;
+                if (t < tl) {
+                    float g[V];
+                    widen<T, V>(rx[u], win[0]);
+                    widen<T, V>(rg[u], g);
+                    if (RESET && fresh[u] != 0) start = t;
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    win[j][e] = win[j - 1][e];
-                    de[j][e] = de[j - 1][e];
+                    for (int e = 0; e < V; ++e) {
+                        float s = bias[e], xw[WM];
+#pragma unroll
+                        for (int j = 0; j < WM; ++j) {
+                            xw[j] = !RESET || t - j >= start ? win[j][e] : 0.f;
+                            s = fmaf(w[j][e], xw[j], s);
+                        }
+                        if (a.silu) {
+                            const float sg = sigmoid(s);
+                            g[e] *= sg * fmaf(s, 1.f - sg, 1.f);
+                        }
+#pragma unroll
+                        for (int j = 0; j < WM; ++j)
+                            if (!RESET || t - j >= start) de[j][e] = fmaf(w[j][e], g[e], de[j][e]);
+                        if (t < t1) {
+                            db[e] += g[e];
+#pragma unroll
+                            for (int j = 0; j < WM; ++j) dw[j][e] = fmaf(xw[j], g[e], dw[j][e]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) win[0][e] = 0.f;
+                }
+                const int q = t - (WM - 1);  // this input has met its last step
+                if ((q >= t0 || (t0 == 0 && q >= -(a.W - 1))) && q < t1) {
+                    const int k = q - (len - (a.W - 1));  // its place in the window after the last step
+                    if (a.dstate_out != nullptr && k >= 0 && k < a.W - 1 && q >= start) {
+                        float r[V];
+                        load_vec<T, V>(static_cast<const T*>(a.dstate_out) + (row * (a.W - 1) + k) * a.d.C + c, r);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) de[WM - 1][e] += r[e];
+                    }
+                    if (q >= 0) store_vec<T, V>(dxp + q * yst, de[WM - 1]);
+                    else if (a.dstate != nullptr) store_vec<T, V>(static_cast<T*>(a.dstate) + (row * (a.W - 1) + a.W - 1 + q) * a.d.C + c, de[WM - 1]);
                 }
 #pragma unroll
-            for (int e = 0; e < V; ++e) de[0][e] = 0.f;
+                for (int j = WM - 1; j > 0; --j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        win[j][e] = win[j - 1][e];
+                        de[j][e] = de[j - 1][e];
+                    }
+#pragma unroll
+                for (int e = 0; e < V; ++e) de[0][e] = 0.f;
+            }
         }
     }
     // the workgroup's rows, in order
-    __shared__ float red[256];
+    __shared__ float red[V][256];
 #pragma unroll
     for (int j = 0; j <= WM; ++j) {
         if (j > a.W - 1 && j != WM) continue;
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            __syncthreads();
-            red[threadIdx.x] = j < WM ? dw[j < WM ? j : 0][e] : db[e];
-            __syncthreads();
-            if (lane_row == 0 && act) {
-                float s = 0.f;
-                for (int k = 0; k < per; ++k) s += red[k * tile + threadIdx.x];
-                const int r = j < WM ? a.W - 1 - j : a.W;
-                a.part[(((int64_t)p * a.slots + blockIdx.y) * (a.W + 1) + r) * a.d.C + c + e] = s;
-            }
+        for (int e = 0; e < V; ++e) red[e][threadIdx.x] = j < WM ? dw[j < WM ? j : 0][e] : db[e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < tile * V; i += 256) {
+            const int cl = i / V, e = i % V, cw = (blockIdx.x % tiles) * tile + cl;
+            if (cw >= CV) continue;
+            float s = 0.f;
+            for (int k = 0; k < per; ++k) s += red[e][k * tile + cl];
+            const int r = j < WM ? a.W - 1 - j : a.W;
+            a.part[(((int64_t)p * a.slots + blockIdx.y) * (a.W + 1) + r) * a.d.C + cw * V + e] = s;
         }
     }
 }
@@ -265,7 +298,13 @@ int conv_validate(const marlhip_ssm_shape* s) {
     return 0;
 }
 
-constexpr int CONV_CHUNK = 16;  // steps of a stretch where the rows alone do not fill the chip
+// Steps of a stretch.  A stretch reads W - 1 inputs (backward: steps) beyond its own, so longer ones cost less, shorter ones give more threads:
+// 16 where that makes 2048 waves of 8 channels a thread, else 8.  Measured: 65536 steps x 1024 channels bf16 forwards 59.7 us with 16, 67.1 with 8;
+// 26 x 1024 rows x 128 channels f32 both ways 30.8 us with 8, 35.3 with 16.
+int conv_chunk(const marlhip_ssm_shape* s) {
+    const int64_t work = (int64_t)s->n_agents * s->batch * s->steps * s->channels;
+    return work >= 16ll * 8 * 64 * 2048 ? 16 : 8;
+}
 
 ConvArgs conv_args(const marlhip_ssm_shape* s, const marlhip_ssm_conv_args* q) {
     ConvArgs a = {};
@@ -275,18 +314,19 @@ ConvArgs conv_args(const marlhip_ssm_shape* s, const marlhip_ssm_conv_args* q) {
     a.weight = q->weight; a.bias = q->bias; a.silu = q->silu != 0;
     a.state = q->state; a.dstate_out = q->dstate_out; a.reset = q->reset; a.lengths = q->lengths;
     a.y = q->y; a.state_out = q->state_out; a.dx = q->dx; a.dstate = q->dstate;
-    a.chunk = CONV_CHUNK;
+    a.chunk = conv_chunk(s);
     a.nchunk = s->steps > 0 ? (s->steps + a.chunk - 1) / a.chunk : 1;
     return a;
 }
 
-// channels a thread takes at once: 16 bytes of them where every pointer and stride allows it
+// channels a thread takes at once where every pointer and stride allows it: 16 bytes of them forwards, 4 of them backwards (its window, its
+// gradients and its sums are kept for each: with 8 they take the whole register file)
 bool aligned(const SsmSeq& q, int v, int e) {
     return q.data == nullptr || ((uintptr_t)q.data % (v * e) == 0 && q.sp % v == 0 && q.st % v == 0 && q.sb % v == 0);
 }
 bool aligned(const void* p, int v, int e) { return (uintptr_t)p % (v * e) == 0; }
-int conv_vec(const ConvArgs& a, int dtype) {
-    const int e = dtype == 0 ? 4 : 2, v = 16 / e;
+int conv_vec(const ConvArgs& a, int dtype, bool grad) {
+    const int e = dtype == 0 ? 4 : 2, v = grad ? 4 : 16 / e;
     const bool ok = a.d.C % v == 0 && aligned(a.x, v, e) && aligned(a.dy, v, e) && aligned(a.state, v, e) && aligned(a.dstate_out, v, e) && aligned(a.y, v, e) &&
                     aligned(a.state_out, v, e) && aligned(a.dx, v, e) && aligned(a.dstate, v, e);
     return ok ? v : 1;
@@ -297,11 +337,16 @@ int conv_tile(int CV) {  // threads along the channels of a backward workgroup
     while (t < CV && t < 64) t *= 2;
     return t;
 }
-int conv_slots(const marlhip_ssm_shape* s) {
-    // the smallest tile any vector width gives: the workspace fits every alignment
-    const int64_t items = (int64_t)s->batch * (s->steps > 0 ? (s->steps + CONV_CHUNK - 1) / CONV_CHUNK : 1);
-    const int64_t cap = 2048 / s->n_agents > 1 ? 2048 / s->n_agents : 1;
+// workgroups that share the rows and stretches of one agent and channel tile
+int conv_slots(const marlhip_ssm_shape* s, int V) {
+    const int chunk = conv_chunk(s), CV = (s->channels + V - 1) / V, tile = conv_tile(CV), tiles = (CV + tile - 1) / tile, per = 256 / tile;
+    const int64_t items = ((int64_t)s->batch * (s->steps > 0 ? (s->steps + chunk - 1) / chunk : 1) + per - 1) / per;
+    const int64_t cap = 2048 / ((int64_t)s->n_agents * tiles) > 1 ? 2048 / ((int64_t)s->n_agents * tiles) : 1;
     return (int)(items < 1 ? 1 : (items < cap ? items : cap));
+}
+int conv_slots_max(const marlhip_ssm_shape* s) {  // whatever the alignment
+    const int a = conv_slots(s, 1), b = conv_slots(s, 4);
+    return a > b ? a : b;
 }
 
 template <class T, int V, int WM, bool RESET>
@@ -310,7 +355,7 @@ int conv_fwd(const ConvArgs& a, hipStream_t st) {
     MARL_REQUIRE(blocks * a.nchunk < (1ll << 31), "ssm_conv: too many rows");
     hipLaunchKernelGGL((ssm_conv_fwd_kernel<T, V, WM, RESET>), dim3((unsigned)(blocks * a.nchunk)), dim3(256), 0, st, a);
     MARL_CHECK_LAUNCH("ssm_conv_fwd_kernel");
-    if (a.nchunk > 1 && a.state_out != nullptr) {
+    if (a.nchunk > 1 && a.state_out != nullptr && a.state_out == a.state) {
         hipLaunchKernelGGL((ssm_conv_window_kernel<T, V, WM>), dim3((unsigned)blocks), dim3(256), 0, st, a);
         MARL_CHECK_LAUNCH("ssm_conv_window_kernel");
     }
@@ -325,20 +370,35 @@ int conv_bwd(const ConvArgs& a, hipStream_t st) {
     return 0;
 }
 
-#define CONV_DISPATCH(fn)                                                                                                        \
-    auto by_reset = [&](auto t, auto v, auto wm) {                                                                               \
-        using T = decltype(t);                                                                                                   \
-        constexpr int V = decltype(v)::v, WM = decltype(wm)::v;                                                                  \
-        return a.reset != nullptr ? fn<T, V, WM, true>(a, st) : fn<T, V, WM, false>(a, st);                                      \
-    };                                                                                                                           \
-    auto by_width = [&](auto t, auto v) { return a.W <= 4 ? by_reset(t, v, Idx<4>{}) : by_reset(t, v, Idx<8>{}); };              \
-    const int vec = conv_vec(a, s->dtype);                                                                                       \
-    if (s->dtype == 0) return vec == 1 ? by_width(float{}, Idx<1>{}) : by_width(float{}, Idx<4>{});                              \
-    if (s->dtype == 1) return vec == 1 ? by_width(__bf16{}, Idx<1>{}) : by_width(__bf16{}, Idx<8>{});                            \
-    return vec == 1 ? by_width(_Float16{}, Idx<1>{}) : by_width(_Float16{}, Idx<8>{});
+template <class F>
+int conv_dispatch(const marlhip_ssm_shape* s, const ConvArgs& a, int vec, F f) {  // f(type, channels a thread, taps, resets)
+    auto by_reset = [&](auto t, auto v, auto wm) { return a.reset != nullptr ? f(t, v, wm, Idx<1>{}) : f(t, v, wm, Idx<0>{}); };
+    auto by_width = [&](auto t, auto v) { return a.W <= 4 ? by_reset(t, v, Idx<4>{}) : by_reset(t, v, Idx<8>{}); };
+    auto by_vec = [&](auto t) {
+        if (vec == 1) return by_width(t, Idx<1>{});
+        if constexpr (sizeof(t) == 2)
+            if (vec == 8) return by_width(t, Idx<8>{});
+        return by_width(t, Idx<4>{});
+    };
+    if (s->dtype == 0) return by_vec(float{});
+    if (s->dtype == 1) return by_vec(__bf16{});
+    return by_vec(_Float16{});
+}
 
-int conv_fwd_any(const marlhip_ssm_shape* s, const ConvArgs& a, hipStream_t st) { CONV_DISPATCH(conv_fwd) }
-int conv_bwd_any(const marlhip_ssm_shape* s, const ConvArgs& a, hipStream_t st) { CONV_DISPATCH(conv_bwd) }
+int conv_fwd_any(const marlhip_ssm_shape* s, const ConvArgs& a, hipStream_t st) {
+    return conv_dispatch(s, a, conv_vec(a, s->dtype, false), [&](auto t, auto v, auto wm, auto re) {
+        constexpr int V = decltype(v)::v;
+        if constexpr (V == 4 && sizeof(t) == 2) return -1;  // 16-bit types take 8 forwards
+        else return conv_fwd<decltype(t), V, decltype(wm)::v, decltype(re)::v != 0>(a, st);
+    });
+}
+int conv_bwd_any(const marlhip_ssm_shape* s, const ConvArgs& a, hipStream_t st) {
+    return conv_dispatch(s, a, conv_vec(a, s->dtype, true), [&](auto t, auto v, auto wm, auto re) {
+        constexpr int V = decltype(v)::v;
+        if constexpr (V == 8) return -1;
+        else return conv_bwd<decltype(t), V, decltype(wm)::v, decltype(re)::v != 0>(a, st);
+    });
+}
 
 }  // namespace
 
@@ -355,7 +415,7 @@ extern "C" int marlhip_ssm_conv(const marlhip_ssm_shape* s, const marlhip_ssm_co
 
 extern "C" int64_t marlhip_ssm_conv_grad_workspace_bytes(const marlhip_ssm_shape* s) {
     if (conv_validate(s) != 0) return -1;
-    return (int64_t)s->n_agents * conv_slots(s) * (s->state + 1) * s->channels * 4;
+    return (int64_t)s->n_agents * conv_slots_max(s) * (s->state + 1) * s->channels * 4;
 }
 
 extern "C" int marlhip_ssm_conv_grad(const marlhip_ssm_shape* s, const marlhip_ssm_conv_args* q, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -367,7 +427,7 @@ extern "C" int marlhip_ssm_conv_grad(const marlhip_ssm_shape* s, const marlhip_s
                  (long long)workspace_bytes);
     ConvArgs a = conv_args(s, q);
     if (a.W == 1) a.dstate_out = nullptr, a.dstate = nullptr;
-    a.slots = conv_slots(s);
+    a.slots = conv_slots(s, conv_vec(a, s->dtype, true));
     a.part = static_cast<float*>(workspace);
     if (conv_bwd_any(s, a, (hipStream_t)stream) != 0) return -1;
     const int64_t cols = (int64_t)(a.W + 1) * a.d.C;
