@@ -537,13 +537,29 @@ __device__ __forceinline__ void put_map(const ScanArgs& a, float v, int64_t om, 
     else static_cast<T*>(i < NP ? a.dB : a.dC)[om + at + n] = down<T>(v);
 }
 
+// the waves' shares of a block's dB and dC, in order
+template <class T, int NP>
+__device__ __forceinline__ void sum_maps(const ScanArgs& a, const float (&red)[WMAX][K * 2 * NP], int64_t om, int64_t pm, int t0, int end, int64_t mst, int nthr) {
+    for (int e = threadIdx.x; e < K * 2 * NP; e += nthr) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WMAX; ++w) v += red[w][e];
+        const int t = t0 + e / (2 * NP);
+        if (t < end) put_map<T, NP>(a, v, om, pm, t * mst, e % (2 * NP));
+    }
+}
+
 // Blocks of K steps from the last to the first: a block's states are recomputed from its record into registers, then its steps run backwards.
 // A workgroup's waves own neighbouring channels of the same rows: they share B and C in LDS and add up their shares of dB and dC there.
 template <class T, int NL, int NS>
 __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) {
     constexpr int NP = NS * NL, KG = K / NS, TOP = 32 / NS;
-    __shared__ float lb[K * NP], lc[K * NP], red[WMAX][K][2 * NP];
+    constexpr bool KEEP = NL == 4;  // decays stay in registers between the two walks over a block: with 8 states a lane there is no room for them
+    // two of each: a block's shares are added up while the next block is worked on, so that one barrier a block does
+    __shared__ float maps_lds[2][2][K * NP], red[2][WMAX][K * 2 * NP];
     const int wv = uni(threadIdx.x >> 6), nthr = a.wpb * 64;
+    for (int i = threadIdx.x; i < 2 * WMAX * K * 2 * NP; i += nthr) (&red[0][0][0])[i] = 0.f;  // waves that this workgroup does not have
+    int buf = 0;
     // workgroup -> (agent, slot, channel group, run of blocks)
     const int gw = a.d.G * a.wgs, ps = uni((int)blockIdx.x / gw), wg = (int)blockIdx.x - ps * gw, p = uni(ps / a.slots), slot = ps - p * a.slots;
     const int grp = uni(wg / a.wgs), run = wg - grp * a.wgs;
@@ -607,6 +623,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
         for (int t0 = tl; t0 >= first && first < end; t0 -= K) {
             float hs[K + 1][NL];                       // hs[s]: the state before step s; hs[K]: after the block
             float x[KG], dt[KG], dys[KG], sd[KG], zv[KG];  // sd: the step size's slope
+            float *lb = maps_lds[buf][0], *lc = maps_lds[buf][1];
             if (wv == 0) store_maps(maps, lb, lc, lane);
             const unsigned fresh = reset_bits(rs);
 #pragma unroll
@@ -623,87 +640,91 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
             }
             __syncthreads();
             if (t0 > first) request(t0 - K);
-#pragma unroll
-            for (int i = 0; i < KG; ++i) {
-                const int out = behind(t0 + i * NS, q.g, end);
-                float dts[NS], us[NS], ys[NS];
-                to_groups<NS>(dt[i], dts);
-                to_groups<NS>(dt[i] * x[i], us);
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    const int s = i * NS + j;
-                    // a reset empties the state through the decay, e^-inf = 0; what is not finite has to go by hand
-                    const bool re = fresh >> s & 1;
-                    const float fr = re ? -INFINITY : 0.f;
-                    if (re) {
-                        asm volatile("");
-#pragma unroll
-                        for (int n = 0; n < NL; ++n) hs[s][n] = fabsf(hs[s][n]) < INFINITY ? hs[s][n] : 0.f;
-                    }
-                    float y = 0.f;
-#pragma unroll
-                    for (int n = 0; n < NL; ++n) {
-                        hs[s + 1][n] = fmaf(exp2_fast(fmaf(dts[j], A[n], fr)), hs[s][n], us[j] * lb[s * NP + q.n0 + n]);
-                        y = fmaf(hs[s + 1][n], lc[s * NP + q.n0 + n], y);
-                    }
-                    ys[j] = y;
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (gated) {
-                    const float y = fmaf(D, x[i], from_groups<NS>(ys)), z = zv[i], sg = sigmoid(z);
-                    row_store(dys[i] * y * sg * fmaf(z, 1.f - sg, 1.f), dzp + (t0 + i * NS) * yst, ROW_MAX, yoff | out);
-                    dys[i] *= z * sg;
-                }
-            }
-            // below, addresses, maps and decays are formed anew: kept from above they would cost more registers than they save time
+            if (t0 < tl) sum_maps<T, NP>(a, red[buf ^ 1], om, pm, t0 + K, end, mst, nthr);
             int t1 = uni(t0);
-            asm volatile("" : "+s"(t1)::"memory");
+            // two forms of the block's steps, as forwards: without resets no step has a branch or a select
+            auto steps = [&](auto plain) __attribute__((always_inline)) {
+                constexpr bool PLAIN = decltype(plain)::v;
+                float ea[KEEP ? K : 1][NL];
 #pragma unroll
-            for (int i = KG - 1; i >= 0; --i) {
-                asm volatile("" : "+v"(dt[i])::"memory");
-                float dts[NS], us[NS], gys[NS], gb[NS], ga[NS];
-                to_groups<NS>(dt[i], dts);
-                to_groups<NS>(dt[i] * x[i], us);
-                to_groups<NS>(dys[i], gys);
+                for (int i = 0; i < KG; ++i) {
+                    const int out = behind(t0 + i * NS, q.g, end);
+                    float dts[NS], us[NS], ys[NS];
+                    to_groups<NS>(dt[i], dts);
+                    to_groups<NS>(dt[i] * x[i], us);
 #pragma unroll
-                for (int j = NS - 1; j >= 0; --j) {
-                    const int s = i * NS + j;
-                    const bool re = fresh >> s & 1;
-                    const float fr = re ? -INFINITY : 0.f;
-                    float sb = 0.f, sa = 0.f;
-                    auto state = [&](auto idx, float& vb, float& vc) __attribute__((always_inline)) {
-                        constexpr int n = decltype(idx)::v;
-                        vc = gys[j] * hs[s + 1][n];  // dC
-                        const float gn = fmaf(gys[j], lc[s * NP + q.n0 + n], dh[n]);
-                        vb = gn * us[j];             // dB
-                        sb = fmaf(gn, lb[s * NP + q.n0 + n], sb);
-                        dh[n] = gn * exp2_fast(fmaf(dts[j], A[n], fr));
-                        const float w = dh[n] * hs[s][n];
-                        sa = fmaf(w, A[n], sa);
-                        dA[n] = fmaf(w, dts[j], dA[n]);
-                    };
-                    const float sum = pair_sums<NL, TOP>(state, lane);
-                    gb[j] = sb;
-                    ga[j] = sa;
-                    if (re) clear(dh);
-                    red[wv][s][(lane / TOP & 1) * NP + q.n0 + (lane / (TOP / NL) & (NL - 1))] = sum;
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int j = 0; j < NS; ++j) {
+                        const int s = i * NS + j;
+                        // a reset empties the state through the decay, e^-inf = 0; what is not finite has to go by hand
+                        const bool re = !PLAIN && (fresh >> s & 1);
+                        const float fr = re ? -INFINITY : 0.f;
+                        int lre = re;
+                        if (!PLAIN) asm volatile("" : "+v"(lre));  // a lane's own flag: a select a state, where the compiler would branch for each
+                        float y = 0.f;
+#pragma unroll
+                        for (int n = 0; n < NL; ++n) {
+                            if (!PLAIN) hs[s][n] = (lre != 0) & !(fabsf(hs[s][n]) < INFINITY) ? 0.f : hs[s][n];
+                            const float ex = exp2_fast(PLAIN ? dts[j] * A[n] : fmaf(dts[j], A[n], fr));
+                            if (KEEP) ea[KEEP ? s : 0][n] = ex;
+                            hs[s + 1][n] = fmaf(ex, hs[s][n], us[j] * lb[s * NP + q.n0 + n]);
+                            y = fmaf(hs[s + 1][n], lc[s * NP + q.n0 + n], y);
+                        }
+                        ys[j] = y;
+                    }
+                    if (gated) {
+                        const float y = fmaf(D, x[i], from_groups<NS>(ys)), z = zv[i], sg = sigmoid(z);
+                        row_store(dys[i] * y * sg * fmaf(z, 1.f - sg, 1.f), dzp + (t0 + i * NS) * yst, ROW_MAX, yoff | out);
+                        dys[i] *= z * sg;
+                    }
                 }
-                const int out = behind(t1 + i * NS, q.g, end);
-                const float b_ = from_groups<NS>(gb), a_ = from_groups<NS>(ga);
-                dD = fmaf(dys[i], x[i], dD);
-                const float dd = out ? 0.f : fmaf(LN2, a_, b_ * x[i]) * sd[i];
-                dbias += dd;
-                row_store(fmaf(dys[i], D, b_ * dt[i]), dxp + (t1 + i * NS) * yst, ROW_MAX, yoff | out);
-                row_store(dd, ddp + (t1 + i * NS) * yst, ROW_MAX, yoff | out);
-            }
+                // below, addresses, maps and (8 states a lane) decays are formed anew: kept from above they would take the registers of a wave
+                asm volatile("" : "+s"(t1)::"memory");
+#pragma unroll
+                for (int i = KG - 1; i >= 0; --i) {
+                    if (!KEEP) asm volatile("" : "+v"(dt[i]));
+                    float dts[NS], us[NS], gys[NS], gb[NS], ga[NS];
+                    to_groups<NS>(dt[i], dts);
+                    to_groups<NS>(dt[i] * x[i], us);
+                    to_groups<NS>(dys[i], gys);
+#pragma unroll
+                    for (int j = NS - 1; j >= 0; --j) {
+                        const int s = i * NS + j;
+                        const bool re = !PLAIN && (fresh >> s & 1);
+                        const float fr = re ? -INFINITY : 0.f;
+                        float sb = 0.f, sa = 0.f;
+                        auto state = [&](auto idx, float& vb, float& vc) __attribute__((always_inline)) {
+                            constexpr int n = decltype(idx)::v;
+                            vc = gys[j] * hs[s + 1][n];  // dC
+                            const float gn = fmaf(gys[j], lc[s * NP + q.n0 + n], dh[n]);
+                            vb = gn * us[j];             // dB
+                            sb = fmaf(gn, lb[s * NP + q.n0 + n], sb);
+                            dh[n] = gn * (KEEP ? ea[KEEP ? s : 0][n] : exp2_fast(PLAIN ? dts[j] * A[n] : fmaf(dts[j], A[n], fr)));
+                            const float w = dh[n] * hs[s][n];
+                            sa = fmaf(w, A[n], sa);
+                            dA[n] = fmaf(w, dts[j], dA[n]);
+                            if (!PLAIN) dh[n] = re ? 0.f : dh[n];
+                        };
+                        const float sum = pair_sums<NL, TOP>(state, lane);
+                        gb[j] = sb;
+                        ga[j] = sa;
+                        red[buf][wv][s * 2 * NP + (lane / TOP & 1) * NP + q.n0 + (lane / (TOP / NL) & (NL - 1))] = sum;
+                    }
+                    const int out = behind(t1 + i * NS, q.g, end);
+                    const float b_ = from_groups<NS>(gb), a_ = from_groups<NS>(ga);
+                    dD = fmaf(dys[i], x[i], dD);
+                    const float dd = out ? 0.f : fmaf(LN2, a_, b_ * x[i]) * sd[i];
+                    dbias += dd;
+                    row_store(fmaf(dys[i], D, b_ * dt[i]), dxp + (t1 + i * NS) * yst, ROW_MAX, yoff | out);
+                    row_store(dd, ddp + (t1 + i * NS) * yst, ROW_MAX, yoff | out);
+                }
+            };
+            if (fresh == 0) steps(Idx<1>{});
+            else steps(Idx<0>{});
+            buf ^= 1;
+        }
+        if (first < end) {
             __syncthreads();
-            for (int e = threadIdx.x; e < K * 2 * NP; e += nthr) {
-                const int s = e / (2 * NP), i = e % (2 * NP);
-                float v = 0.f;
-                for (int w = 0; w < a.wpb; ++w) v += red[w][s][i];
-                if (t1 + s < end) put_map<T, NP>(a, v, om, pm, (t1 + s) * mst, i);
-            }
+            sum_maps<T, NP>(a, red[buf ^ 1], om, pm, first, end, mst, nthr);
         }
         if (a.dh_in != nullptr && ch == 0) store_state(a, q, a.dh_in + (int64_t)row * N * C, dh);
     }
