@@ -8,7 +8,6 @@
 // shares of y.  So NS > 1 costs three swaps a step, keeps 8 / N of the registers and gives NS times the waves, which is what small batches need.
 // B and C of a step are the same for a group's channels and come as LDS broadcasts, K steps at a time.
 #include "ssm.h"
-#include <stdlib.h>
 
 using namespace marl;
 
@@ -771,13 +770,15 @@ struct ScanPlan {
     int NL, NS, nblk, chunk, nchunk, nck, wpb, wgs, slots;
 };
 
-// How a call is split.  One wave a SIMD (1024 of them) is where the chip begins to be filled.  Batches that stay below keep 4 states a lane
-// instead of 8 (twice the waves for a sixth more instructions); a sequence of still fewer is cut into chunks, which costs a first pass over
-// delta, x and B (or dy, C) of about 0.8 of the second one.
+// How a call is split.  A row of N states a channel takes N / 8 x C / 64 waves with 8 states a lane; the chip has 1024 SIMDs and wants about
+// four waves on each.
+//   <= 512 waves and long enough: the sequences are cut into chunks of at least 64 steps for 4096 waves.  That costs a first pass of about 0.8
+//     of the second (16384 steps x 512 channels bf16: 12300 us in one piece, 33 + 12 + 43 us in 256 chunks).
+//   <= 1024 waves otherwise: 4 states a lane, twice the waves for a sixth more instructions (501 steps x 128 rows x 256 channels bf16: forwards
+//     146 -> 120 us; cut into 4 chunks 158.  Backwards 582 -> 388; cut 376.  With 2048 waves 8 a lane are better: 74 against 80 us).
 ScanPlan scan_plan(const marlhip_ssm_shape* s) {
-    static const int TGT = getenv("SSM_T") ? atoi(getenv("SSM_T")) : 4096, THR = getenv("SSM_H") ? atoi(getenv("SSM_H")) : 512, MINC = getenv("SSM_C") ? atoi(getenv("SSM_C")) : 64;
-    static const int WM = getenv("SSM_W") ? atoi(getenv("SSM_W")) : WMAX;
-    static const int N4 = getenv("SSM_N4") ? atoi(getenv("SSM_N4")) : 1024;
+    constexpr int64_t CUT_WAVES = 512, FEW_WAVES = 1024, WANT_WAVES = 4096;
+    constexpr int CUT_STEPS = 64;
     ScanPlan q;
     const int Cg = s->channels / s->groups;
     auto lanes = [&](int nl, int ns) {
@@ -786,26 +787,27 @@ ScanPlan scan_plan(const marlhip_ssm_shape* s) {
         q.nblk = (Cg + 64 / ns - 1) / (64 / ns);
         return (int64_t)s->n_agents * s->batch * s->groups * q.nblk;
     };
-    int64_t waves;
-    if (s->state <= 4) waves = lanes(4, 1);
-    else if (s->state <= 8) waves = lanes(8, 1) <= N4 ? lanes(4, 2) : lanes(8, 1);
-    else if (s->state <= 16) waves = lanes(8, 2) <= N4 ? lanes(4, 4) : lanes(8, 2);
-    else waves = lanes(8, 4);
+    const bool cuts = s->steps >= 2 * CUT_STEPS;
+    auto choose = [&](int nl, int ns) {
+        const int64_t w = lanes(nl, ns);
+        return w > FEW_WAVES || (cuts && w <= CUT_WAVES) ? w : lanes(nl / 2, ns * 2);
+    };
+    const int64_t waves = s->state <= 4 ? lanes(4, 1) : (s->state <= 8 ? choose(8, 1) : (s->state <= 16 ? choose(8, 2) : lanes(8, 4)));
     q.nck = (s->steps + K - 1) / K;
     q.nchunk = 1;
     q.chunk = q.nck > 0 ? q.nck * K : K;
-    if (waves > 0 && waves <= THR && s->steps >= 2 * MINC) {
-        int64_t want = TGT / waves, most = s->steps / MINC;
-        if (want > most) want = most;
-        if (want > 1) {
-            q.chunk = (int)((q.nck + want - 1) / want) * K;
+    if (waves > 0 && waves <= CUT_WAVES && cuts) {
+        const int64_t want = WANT_WAVES / waves, most = s->steps / CUT_STEPS;
+        const int64_t n = want < most ? want : most;
+        if (n > 1) {
+            q.chunk = (int)((q.nck + n - 1) / n) * K;
             q.nchunk = (s->steps + q.chunk - 1) / q.chunk;
         }
     }
-    q.wpb = q.nblk < WM ? q.nblk : WM;
+    q.wpb = q.nblk < WMAX ? q.nblk : WMAX;
     q.wgs = (q.nblk + q.wpb - 1) / q.wpb;
-    // items of one agent that a backward workgroup takes one after the other (its sums over them stay in registers)
-    const int64_t items = (int64_t)s->batch * q.nchunk, k = 4096 / ((int64_t)s->n_agents * s->groups * q.wgs * q.wpb);
+    // items of one agent that a backward workgroup takes one after the other (its sums over them stay in registers): 4096 waves for them all
+    const int64_t items = (int64_t)s->batch * q.nchunk, k = WANT_WAVES / ((int64_t)s->n_agents * s->groups * q.wgs * q.wpb);
     q.slots = (int)(items < 1 ? 1 : (items < k ? items : (k < 1 ? 1 : k)));
     return q;
 }

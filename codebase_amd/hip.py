@@ -1362,25 +1362,40 @@ def _dense(what, name, t, shape, dtype, dev):
     """address of a contiguous argument (0: absent)"""
     if t is None:
         return 0
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
-        _expect(what, name, t, shape, dtype, dev)
-    return t.data_ptr()
+    try:
+        if t.shape == shape and t.dtype is dtype and t.get_device() == dev and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _expect(what, name, t, shape, dtype, dev)
 
 
 def _seq(what, name, t, shape, dtype, dev):
-    """marlhip_ssm_seq of a sequence or a map"""
+    """marlhip_ssm_seq of a sequence"""
     if t is None:
         return _NO_SEQ
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
-        _expect(what, name, t, shape, dtype, dev, dense=False)
-    st = t.stride()
-    if st[-1] != 1 or len(shape) == 5:
-        step = 1
-        for d in range(len(shape) - 1, 2, -1):  # channels, or a map's groups and states
-            if shape[d] != 1 and st[d] != step and t.numel():
-                raise ValueError(f"{what}: {name} has stride {st[d]} in dimension {d}, expected {step}")
-            step *= shape[d]
-    return t.data_ptr(), st[0], st[1], st[2]
+    try:
+        if t.shape == shape and t.dtype is dtype and t.get_device() == dev:
+            sp, st, sb, sc = t.stride()
+            if sc == 1 or shape[3] == 1 or not t.numel():
+                return t.data_ptr(), sp, st, sb
+            raise ValueError(f"{what}: {name} has stride {sc} in dimension 3, expected 1")
+    except AttributeError:
+        pass
+    _expect(what, name, t, shape, dtype, dev, dense=False)
+
+
+def _map(what, name, t, shape, dtype, dev):
+    """marlhip_ssm_seq of a map [P][S][B][G][N], dense in groups and states"""
+    try:
+        if t.shape == shape and t.dtype is dtype and t.get_device() == dev:
+            sp, st, sb, sg, sn = t.stride()
+            if (sn == 1 or shape[4] == 1) and (sg == shape[4] or shape[3] == 1) or not t.numel():
+                return t.data_ptr(), sp, st, sb
+            raise ValueError(f"{what}: {name} has stride {(sg, sn)} in its last dimensions, expected {(shape[4], 1)}")
+    except AttributeError:
+        pass
+    _expect(what, name, t, shape, dtype, dev, dense=False)
 
 
 def _ssm_shape(what, x, state, groups, sharing):
@@ -1430,12 +1445,23 @@ def _in_place_or_apart(what, name, out, src):
         raise ValueError(f"{what}: {name} overlaps the state that the call reads")
 
 
-def _launch(what, dev, call):
-    """call(raw stream) with the tensors' device current: on that device's current stream"""
-    if torch._C._cuda_getDevice() == dev:
-        return call(torch._C._cuda_getCurrentRawStream(dev))
-    with torch.cuda.device(dev):
-        return call(torch._C._cuda_getCurrentRawStream(dev))
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream if torch.cuda._is_compiled() else None, torch.cuda.current_device
+
+
+def _call(what, fn, dev, *args):
+    """fn(*args, stream) with the tensors' device current, on that device's current stream"""
+    if _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc < 0:
+        check(rc, what)
+
+
+def _dense_like(t):
+    """an uninitialised contiguous tensor of t's shape and type (None for None)"""
+    return None if t is None else torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _need_device(what, t, dev):
@@ -1466,13 +1492,12 @@ def ssm_conv(x, weight, bias=None, silu=True, sharing=None, state=None, want_sta
     so = _dense("ssm_conv", "state_out", state_out, window, x.dtype, dev)
     _in_place_or_apart("ssm_conv", "state_out", state_out, state)
     _need_device("ssm_conv", x, dev)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     if want_state and state_out is None:
         state_out = torch.empty(window, dtype=x.dtype, device=x.device)
         so = state_out.data_ptr()
     args = _CONV_PACK(*xs, *_NO_SEQ, w, b, 1 if silu else 0, st, rs, ln, y.data_ptr(), so, 0, 0, 0, 0, 0)
-    if _launch("ssm_conv", dev, lambda stream: lib.marlhip_ssm_conv(shape, args, stream)) < 0:
-        check(-1, "ssm_conv")
+    _call("ssm_conv", lib.marlhip_ssm_conv, dev, shape, args)
     return (y, state_out) if want_state else y
 
 
@@ -1480,16 +1505,16 @@ def ssm_conv_grad(dy, x, weight, bias=None, silu=True, sharing=None, state=None,
     """gradients of ssm_conv for the same arguments: dy [P][S][B][C] at y and (optional) dstate_out [P][B][W-1][C] at state_out ->
     SsmConvGrad(x, weight, bias, state); bias / state are None where the argument is"""
     shape, dev, xs, w, b, st, rs, ln, window = _conv_args("ssm_conv_grad", x, weight, bias, sharing, state, reset, lengths)
+    if dy is None:
+        raise ValueError("ssm_conv_grad: dy is not a tensor")
     dys = _seq("ssm_conv_grad", "dy", dy, x.shape, x.dtype, dev)
     dso = _dense("ssm_conv_grad", "dstate_out", dstate_out, window, x.dtype, dev)
     _need_device("ssm_conv_grad", x, dev)
     n = _ssm_size(lib.marlhip_ssm_conv_grad_workspace_bytes, "ssm_conv_grad_workspace_bytes", shape)
-    g = SsmConvGrad(torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(weight),
-                    None if bias is None else torch.empty_like(bias), None if state is None else torch.empty_like(state))
+    g = SsmConvGrad(_dense_like(x), _dense_like(weight), _dense_like(bias), _dense_like(state))
     ws = torch.empty(n, dtype=torch.uint8, device=x.device)
     args = _CONV_PACK(*xs, *dys, w, b, 1 if silu else 0, st, rs, ln, 0, 0, dso, *(0 if t is None else t.data_ptr() for t in (g.x, g.state, g.weight, g.bias)))
-    if _launch("ssm_conv_grad", dev, lambda stream: lib.marlhip_ssm_conv_grad(shape, args, ws.data_ptr(), n, stream)) < 0:
-        check(-1, "ssm_conv_grad")
+    _call("ssm_conv_grad", lib.marlhip_ssm_conv_grad, dev, shape, args, ws.data_ptr(), n)
     return g
 
 
@@ -1503,10 +1528,10 @@ def _scan_args(what, x, delta, A, B, C, D, z, delta_bias, sharing, h_in, reset, 
     shape, M, dev = _ssm_shape(what, x, N, G, sharing)
     P, S, NB, Ch = xshape = x.shape
     dt, mshape, hshape = x.dtype, (P, S, NB, G, N), (P, NB, N, Ch)
-    seqs = (_seq(what, "x", x, xshape, dt, dev) + _seq(what, "delta", delta, xshape, dt, dev) + _seq(what, "B", B, mshape, dt, dev)
-            + _seq(what, "C", C, mshape, dt, dev) + _seq(what, "z", z, xshape, dt, dev))
-    if delta is None or C is None:
-        raise ValueError(f"{what}: delta and C are not optional")
+    if delta is None:
+        raise ValueError(f"{what}: delta is not a tensor")
+    seqs = (_seq(what, "x", x, xshape, dt, dev) + _seq(what, "delta", delta, xshape, dt, dev) + _map(what, "B", B, mshape, dt, dev)
+            + _map(what, "C", C, mshape, dt, dev) + _seq(what, "z", z, xshape, dt, dev))
     rec = 0
     if record is not None:
         rec = _dense(what, "record", record, (_ssm_size(lib.marlhip_ssm_scan_record_floats, "ssm_scan_record_floats", shape),), _F32, dev)
@@ -1534,14 +1559,13 @@ def ssm_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=True, 
     _in_place_or_apart("ssm_scan", "h_out", h_out, h_in)
     _need_device("ssm_scan", x, dev)
     n = _ssm_size(lib.marlhip_ssm_scan_workspace_bytes, "ssm_scan_workspace_bytes", shape)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     if want_h and h_out is None:
         h_out = torch.empty(hshape, dtype=_F32, device=x.device)
         ho = h_out.data_ptr()
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device).data_ptr() if n else 0
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
     args = _SCAN_PACK(*seqs, *_NO_SEQ, pA, pD, pb, 1 if softplus else 0, ph, rs, ln, y.data_ptr(), ho, rec, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    if _launch("ssm_scan", dev, lambda stream: lib.marlhip_ssm_scan(shape, args, ws, n, stream)) < 0:
-        check(-1, "ssm_scan")
+    _call("ssm_scan", lib.marlhip_ssm_scan, dev, shape, args, 0 if ws is None else ws.data_ptr(), n)
     return (y, h_out) if want_h else y
 
 
@@ -1553,19 +1577,16 @@ def ssm_scan_grad(dy, x, delta, A, B, C, record, D=None, z=None, delta_bias=None
     shape, dev, hshape, seqs, pA, pD, pb, ph, rs, ln, rec = _scan_args(what, x, delta, A, B, C, D, z, delta_bias, sharing, h_in, reset, lengths, record)
     if record is None:
         raise ValueError("ssm_scan_grad: record is missing (ssm_scan fills it: record=ssm_scan_record(x, n_states))")
+    if dy is None:
+        raise ValueError(f"{what}: dy is not a tensor")
     dys, dho = _seq(what, "dy", dy, x.shape, x.dtype, dev), _dense(what, "dh_out", dh_out, hshape, _F32, dev)
     _need_device(what, x, dev)
     n = _ssm_size(lib.marlhip_ssm_scan_grad_workspace_bytes, "ssm_scan_grad_workspace_bytes", shape)
-
-    def like(t):
-        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-    g = SsmScanGrad(like(x), like(delta), like(A), like(B), like(C), like(D), like(z), like(delta_bias), like(h_in))
+    g = SsmScanGrad(*map(_dense_like, (x, delta, A, B, C, D, z, delta_bias, h_in)))
     ws = torch.empty(n, dtype=torch.uint8, device=x.device)
     out = (0 if t is None else t.data_ptr() for t in (g.x, g.delta, g.B, g.C, g.z, g.A, g.D, g.delta_bias, g.h_in))
     args = _SCAN_PACK(*seqs, *dys, pA, pD, pb, 1 if softplus else 0, ph, rs, ln, 0, 0, rec, dho, *out)
-    if _launch(what, dev, lambda stream: lib.marlhip_ssm_scan_grad(shape, args, ws.data_ptr(), n, stream)) < 0:
-        check(-1, what)
+    _call(what, lib.marlhip_ssm_scan_grad, dev, shape, args, ws.data_ptr(), n)
     return g
 
 
@@ -1619,7 +1640,7 @@ def grad_norm(tensors):
     _need_device("grad_norm", first, dev)
     nb = check(lib.marlhip_grad_norm_workspace_bytes(table, count), "grad_norm_workspace_bytes")
     norm, ws = torch.empty(1, dtype=_F32, device=first.device), torch.empty(nb, dtype=torch.uint8, device=first.device)
-    check(_launch("grad_norm", dev, lambda stream: lib.marlhip_grad_norm(table, count, norm.data_ptr(), ws.data_ptr(), nb, stream)), "grad_norm")
+    _call("grad_norm", lib.marlhip_grad_norm, dev, table, count, norm.data_ptr(), ws.data_ptr(), nb)
     return norm
 
 
@@ -1636,5 +1657,5 @@ def clip_grad_norm(tensors, max_norm, out=None):
     _need_device("clip_grad_norm", first, dev)
     nb = check(lib.marlhip_grad_norm_workspace_bytes(table, count), "grad_norm_workspace_bytes")
     norm, ws = torch.empty(1, dtype=_F32, device=first.device), torch.empty(nb, dtype=torch.uint8, device=first.device)
-    check(_launch("clip_grad_norm", dev, lambda stream: lib.marlhip_clip_grad_norm(table, count, max_norm, norm.data_ptr(), ws.data_ptr(), nb, stream)), "clip_grad_norm")
+    _call("clip_grad_norm", lib.marlhip_clip_grad_norm, dev, table, count, max_norm, norm.data_ptr(), ws.data_ptr(), nb)
     return norm
