@@ -299,11 +299,12 @@ int conv_validate(const marlhip_ssm_shape* s) {
 }
 
 // Steps of a stretch.  A stretch reads W - 1 inputs (backward: steps) beyond its own, so longer ones cost less, shorter ones give more threads:
-// 16 where that makes 2048 waves of 8 channels a thread, else 8.  Measured: 65536 steps x 1024 channels bf16 forwards 59.7 us with 16, 67.1 with 8;
-// 26 x 1024 rows x 128 channels f32 both ways 30.8 us with 8, 35.3 with 16.
+// the longest of 32, 16 and 8 that makes 2048 waves of 8 channels a thread, or 8.  Measured: 65536 steps x 1024 channels bf16 forwards 66 us with
+// 32, 69 with 16, 77 with 8; 26 x 1024 rows x 128 channels f32 both ways 30.8 us with 8, 35.3 with 16, 43 with 32.
 int conv_chunk(const marlhip_ssm_shape* s) {
     const int64_t work = (int64_t)s->n_agents * s->batch * s->steps * s->channels;
-    return work >= 16ll * 8 * 64 * 2048 ? 16 : 8;
+    constexpr int64_t WAVES = 8ll * 64 * 2048;
+    return work >= 32 * WAVES ? 32 : (work >= 16 * WAVES ? 16 : 8);
 }
 
 ConvArgs conv_args(const marlhip_ssm_shape* s, const marlhip_ssm_conv_args* q) {

@@ -662,7 +662,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                         float y = 0.f;
 #pragma unroll
                         for (int n = 0; n < NL; ++n) {
-                            if (!PLAIN) hs[s][n] = (lre != 0) & !(fabsf(hs[s][n]) < INFINITY) ? 0.f : hs[s][n];
+                            if (!PLAIN) hs[s][n] = ((lre != 0) & !(fabsf(hs[s][n]) < INFINITY)) ? 0.f : hs[s][n];
                             const float ex = exp2_fast(PLAIN ? dts[j] * A[n] : fmaf(dts[j], A[n], fr));
                             if (KEEP) ea[KEEP ? s : 0][n] = ex;
                             hs[s + 1][n] = fmaf(ex, hs[s][n], us[j] * lb[s * NP + q.n0 + n]);
