@@ -23,6 +23,9 @@ struct ConvArgs {
 
 constexpr int U = 4;  // steps requested together
 
+// Kernels for 2, 3, 4 and up to 8 taps (WM); a tap that is not there is left out, not multiplied by 0, which an infinity would show
+#define HAS_TAP(j) (WM < 8 || (j) < a.W)
+
 template <class T, int V>
 struct alignas(V * sizeof(T)) Vec {
     T v[V];
@@ -136,9 +139,11 @@ __global__ __launch_bounds__(256) void ssm_conv_fwd_kernel(ConvArgs a) {
             for (int e = 0; e < V; ++e) {
                 float s = bias[e];
 #pragma unroll
-                for (int j = 0; j < WM; ++j)
+                for (int j = 0; j < WM; ++j) {
+                    if (!HAS_TAP(j)) continue;
                     if (!RESET || j == 0) s = fmaf(w[j][e], win[j][e], s);
                     else s = t + u - j >= start ? fmaf(w[j][e], win[j][e], s) : s;
+                }
                 y[e] = t + u < len ? (a.silu ? s * sigmoid(s) : s) : 0.f;
             }
 #pragma unroll
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(256) void ssm_conv_bwd_kernel(ConvArgs a, int tile)
 #pragma unroll
                         for (int j = 0; j < WM; ++j) {
                             xw[j] = !RESET || t - j >= start ? win[j][e] : 0.f;
-                            s = fmaf(w[j][e], xw[j], s);
+                            if (HAS_TAP(j)) s = fmaf(w[j][e], xw[j], s);
                         }
                         if (a.silu) {
                             const float sg = sigmoid(s);
@@ -236,7 +241,7 @@ __global__ __launch_bounds__(256) void ssm_conv_bwd_kernel(ConvArgs a, int tile)
                         }
 #pragma unroll
                         for (int j = 0; j < WM; ++j)
-                            if (!RESET || t - j >= start) de[j][e] = fmaf(w[j][e], g[e], de[j][e]);
+                            if (HAS_TAP(j) && (!RESET || t - j >= start)) de[j][e] = fmaf(w[j][e], g[e], de[j][e]);
                         if (t < t1) {
                             db[e] += g[e];
 #pragma unroll
@@ -275,7 +280,7 @@ __global__ __launch_bounds__(256) void ssm_conv_bwd_kernel(ConvArgs a, int tile)
     __shared__ float red[V][256];
 #pragma unroll
     for (int j = 0; j <= WM; ++j) {
-        if (j > a.W - 1 && j != WM) continue;
+        if (j != WM && !HAS_TAP(j)) continue;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < V; ++e) red[e][threadIdx.x] = j < WM ? dw[j < WM ? j : 0][e] : db[e];
@@ -374,7 +379,12 @@ int conv_bwd(const ConvArgs& a, hipStream_t st) {
 template <class F>
 int conv_dispatch(const marlhip_ssm_shape* s, const ConvArgs& a, int vec, F f) {  // f(type, channels a thread, taps, resets)
     auto by_reset = [&](auto t, auto v, auto wm) { return a.reset != nullptr ? f(t, v, wm, Idx<1>{}) : f(t, v, wm, Idx<0>{}); };
-    auto by_width = [&](auto t, auto v) { return a.W <= 4 ? by_reset(t, v, Idx<4>{}) : by_reset(t, v, Idx<8>{}); };
+    auto by_width = [&](auto t, auto v) {
+        if (a.W == 4) return by_reset(t, v, Idx<4>{});
+        if (a.W == 3) return by_reset(t, v, Idx<3>{});
+        if (a.W == 2) return by_reset(t, v, Idx<2>{});
+        return by_reset(t, v, Idx<8>{});
+    };
     auto by_vec = [&](auto t) {
         if (vec == 1) return by_width(t, Idx<1>{});
         if constexpr (sizeof(t) == 2)
@@ -424,7 +434,7 @@ extern "C" int marlhip_ssm_conv_grad(const marlhip_ssm_shape* s, const marlhip_s
     MARL_REQUIRE(q != nullptr && q->weight != nullptr && q->dweight != nullptr, "ssm_conv_grad: NULL argument");
     MARL_REQUIRE(s->steps == 0 || s->batch == 0 || (q->x.data && q->dy.data && q->dx), "ssm_conv_grad: NULL pointer");
     const int64_t need = marlhip_ssm_conv_grad_workspace_bytes(s);
-    MARL_REQUIRE(workspace != nullptr && workspace_bytes >= need, "ssm_conv_grad: workspace of %lld bytes needed, %lld given", (long long)need,
+    MARL_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need, "ssm_conv_grad: aligned workspace of %lld bytes needed, %lld given", (long long)need,
                  (long long)workspace_bytes);
     ConvArgs a = conv_args(s, q);
     if (a.W == 1) a.dstate_out = nullptr, a.dstate = nullptr;

@@ -814,18 +814,17 @@ ScanPlan scan_plan(const marlhip_ssm_shape* s) {
 
 int64_t scan_items(const marlhip_ssm_shape* s, const ScanPlan& pl) { return (int64_t)s->n_agents * s->batch * pl.nchunk * s->groups * pl.nblk; }
 
-int seq_check(const char* what, const char* name, const marlhip_ssm_seq& q, int esize, int64_t steps) {
-    // a wave addresses up to 4 steps with 32-bit offsets
-    MARL_REQUIRE(q.data == nullptr || steps <= 1 || (q.step_stride >= 0 && q.step_stride * esize <= (1ll << 29)),
-                 "%s: %s has %lld elements between steps (0..2^29 bytes supported)", what, name, (long long)q.step_stride);
+int seq_check(const char* what, const char* name, const marlhip_ssm_seq& q, int esize, int64_t steps, int log_bytes) {
+    MARL_REQUIRE(q.data == nullptr || steps <= 1 || (q.step_stride >= 0 && q.step_stride <= (1ll << log_bytes) / esize),
+                 "%s: %s has %lld elements between steps (0..2^%d bytes supported)", what, name, (long long)q.step_stride, log_bytes);
     return 0;
 }
 int scan_seqs(const char* what, const marlhip_ssm_shape* s, const marlhip_ssm_scan_args* q, bool grad) {
     const int e = s->dtype == 0 ? 4 : 2;
-    if (seq_check(what, "x", q->x, e, s->steps) || seq_check(what, "delta", q->delta, e, s->steps) || seq_check(what, "z", q->z, e, s->steps)) return -1;
-    if (grad && seq_check(what, "dy", q->dy, e, s->steps)) return -1;
-    // the maps' offsets run over K steps: half the span
-    if (seq_check(what, "B", q->B, 2 * e, s->steps) || seq_check(what, "C", q->C, 2 * e, s->steps)) return -1;
+    // 32-bit offsets run over up to 4 steps of a sequence, over 8 of a map
+    if (seq_check(what, "x", q->x, e, s->steps, 29) || seq_check(what, "delta", q->delta, e, s->steps, 29) || seq_check(what, "z", q->z, e, s->steps, 29)) return -1;
+    if (grad && seq_check(what, "dy", q->dy, e, s->steps, 29)) return -1;
+    if (seq_check(what, "B", q->B, e, s->steps, 28) || seq_check(what, "C", q->C, e, s->steps, 28)) return -1;
     MARL_REQUIRE(scan_items(s, scan_plan(s)) < (1ll << 31) - 8, "%s: batch %d x channels %d is too large", what, s->batch, s->channels);
     MARL_REQUIRE(s->steps <= 1 || (int64_t)s->batch * s->channels * e <= (1ll << 29), "%s: batch %d x channels %d: a step is over 2^29 bytes", what, s->batch,
                  s->channels);
@@ -933,8 +932,8 @@ extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_sc
     if (scan_seqs("ssm_scan", s, q, false) != 0) return -1;
     const ScanPlan pl = scan_plan(s);
     const CarryWs w = carry_ws(s, pl);
-    MARL_REQUIRE(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total), "ssm_scan: workspace of %lld bytes needed, %lld given", (long long)w.total,
-                 (long long)workspace_bytes);
+    MARL_REQUIRE(w.total == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= w.total),
+                 "ssm_scan: aligned workspace of %lld bytes needed, %lld given", (long long)w.total, (long long)workspace_bytes);
     if (s->batch == 0) return 0;
     ScanArgs a = scan_args(s, q, pl);
     if (s->steps == 1 && a.record == nullptr) return scan_step(s, a, (hipStream_t)stream);
@@ -991,8 +990,8 @@ extern "C" int marlhip_ssm_scan_grad(const marlhip_ssm_shape* s, const marlhip_s
     if (scan_seqs("ssm_scan_grad", s, q, true) != 0) return -1;
     const ScanPlan pl = scan_plan(s);
     const GradWs w = grad_ws(s, pl);
-    MARL_REQUIRE(workspace != nullptr && workspace_bytes >= w.total, "ssm_scan_grad: workspace of %lld bytes needed, %lld given", (long long)w.total,
-                 (long long)workspace_bytes);
+    MARL_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= w.total,
+                 "ssm_scan_grad: aligned workspace of %lld bytes needed, %lld given", (long long)w.total, (long long)workspace_bytes);
     ScanArgs a = scan_args(s, q, pl);
     char* ws = static_cast<char*>(workspace);
     hipStream_t st = (hipStream_t)stream;

@@ -1474,6 +1474,8 @@ def _conv_args(what, x, weight, bias, sharing, state, reset, lengths):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
         raise ValueError(f"{what}: weight is not a [networks][taps][channels] tensor")
     W = weight.shape[1]
+    if not 1 <= W <= 8:
+        raise ValueError(f"{what}: {W} taps (1..8 supported)")
     shape, M, dev = _ssm_shape(what, x, W, 1, sharing)
     P, _, B, C = x.shape
     window = (P, B, W - 1, C)

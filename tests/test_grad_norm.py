@@ -72,6 +72,12 @@ def test_unaligned_views_and_shapes(dtype):
 
 
 @pytest.mark.gpu
+def test_tensors_without_elements():
+    ts = [torch.zeros(0, device="cuda"), torch.zeros(3, 0, dtype=torch.bfloat16, device="cuda")]
+    assert h.grad_norm(ts).item() == 0.0 and h.clip_grad_norm(ts, 1.0).item() == 0.0
+
+
+@pytest.mark.gpu
 def test_large_and_small_values():
     ts = [torch.full((1000,), 3e30, device="cuda"), torch.full((10,), 1e-30, device="cuda")]
     assert abs(h.grad_norm(ts).item() / (3e30 * math.sqrt(1000)) - 1) <= 2 * U  # the squares pass an f32's range

@@ -524,6 +524,47 @@ def test_conv_does_not_look_behind_the_end_or_a_reset(bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("W", [1, 2, 3, 4, 5, 7, 8])
+def test_conv_looks_at_its_taps_alone(W, bad):
+    """what is not finite reaches the W steps whose window holds it, and the W inputs of a step whose gradient is not"""
+    S, at = 37, 11
+    v = make_conv(1, S, 3, 12, W, reset=False, lengths=False)
+    y, g = conv_call(v), conv_grad_call(v)
+    w = dict(v, x=v["x"].clone())
+    w["x"][:, at] = bad
+    y1, g1 = conv_call(w), conv_grad_call(w)
+    far = [t for t in range(S) if not at <= t < at + W]
+    assert torch.equal(y[:, far], y1[:, far]) and not torch.isfinite(y1[:, at:at + W]).any()
+    near = range(max(0, at - W + 1), at + W)  # inputs of a step whose slope is not finite
+    assert torch.equal(g.x[:, [t for t in range(S) if t not in near]], g1.x[:, [t for t in range(S) if t not in near]])
+    w = dict(v, dy=v["dy"].clone())
+    w["dy"][:, at] = bad
+    g2 = conv_grad_call(w)
+    far = [t for t in range(S) if not at - W < t <= at]
+    assert torch.equal(g.x[:, far], g2.x[:, far])
+
+
+@pytest.mark.gpu
+def test_conv_gradient_against_differences():
+    v = make_conv(2, 9, 3, 10, 4, lengths=False)
+    g = conv_grad_call(v)
+
+    def loss(w):
+        ref = conv_reference(w, grads=False)
+        return ((ref["y"][0] * v["dy"].double()).sum() + (ref["state"][0] * v["dstate_out"].double()).sum()).item()
+
+    for name, grad in dict(x=g.x, weight=g.weight, bias=g.bias, state=g.state).items():
+        d = grad.double()
+        step = 1e-4 / max(d.abs().max().item(), 1.0)
+        plus, minus = dict(v), dict(v)
+        plus[name], minus[name] = v[name].double() + step * d, v[name].double() - step * d
+        slope, want = (loss(plus) - loss(minus)) / (2 * step), (d * d).sum().item()
+        # as for the scan: third derivatives times step^2 / 6, and the gradient's own 64 roundings
+        assert abs(slope - want) <= 1e-4 * abs(want), (name, slope, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_conv_step_by_step_in_place(dtype):
     v = make_conv(2, 14, 6, 80, 4, dtype=dtype, lengths=False)
@@ -869,6 +910,9 @@ def test_conv_refuses_states_and_the_cpu():
         conv_grad_call(dict(v, dstate_out=v["state"][:1]))
     with pytest.raises(h.MarlHipError, match="CPU"):
         conv_call(v)
+    for W in (0, 9):
+        with pytest.raises(ValueError, match=f"{W} taps"):
+            h.ssm_conv(v["x"], torch.empty(2, W, 12))
     with pytest.raises(h.MarlHipError, match="9 taps"):
         import ctypes
 
