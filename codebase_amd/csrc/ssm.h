@@ -92,19 +92,11 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // 2^v on the transcendental unit (results below 2^-126 become 0: a decay that small has emptied the state either way)
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * v)); }
-// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| <= 1, by log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the odd series up to s^15
-// is off by less than s^16 / 17 < 2e-9 of the value for every e, where a logarithm of the rounded 1 + e loses what a small e says
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| <= 1.  What rounding u = 1 + e lost of e, c = e - (u - 1), is added to log u.  The exact term is
+// c / u: with |c| <= 2^-24 u the difference |c - c / u| = |c| e / u is at most 2^-24 e, a step and a half of log(1 + e) >= e log 2.
 __device__ __forceinline__ float softplus(float v) {
-    const float e = exp2_fast(-LOG2E * fabsf(v)), s = e * __builtin_amdgcn_rcpf(2.f + e), w = s * s;
-    float q = 1.f / 15.f;
-    q = fmaf(q, w, 1.f / 13.f);
-    q = fmaf(q, w, 1.f / 11.f);
-    q = fmaf(q, w, 1.f / 9.f);
-    q = fmaf(q, w, 1.f / 7.f);
-    q = fmaf(q, w, 1.f / 5.f);
-    q = fmaf(q, w, 1.f / 3.f);
-    q = fmaf(q, w, 1.f);
-    return fmaf(2.f * s, q, fmaxf(v, 0.f));
+    const float e = exp2_fast(-LOG2E * fabsf(v)), u = 1.f + e;
+    return fmaxf(v, 0.f) + fmaf(LN2, __builtin_amdgcn_logf(u), e - (u - 1.f));
 }
 
 // ---- sums over a wave's lanes ----------------------------------------------------------------------------------------------------
