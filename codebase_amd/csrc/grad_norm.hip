@@ -3,7 +3,7 @@
 // The tensors' pointers travel in the kernel's own arguments, up to 160 a launch: no table has to be copied to the device, and a captured
 // graph holds them.  A first pass leaves one 64-bit sum of squares a workgroup, a second one adds them up in every workgroup (the same order
 // everywhere) and scales, in the opposite direction: what the first pass read last is still in the caches.  Bound by HBM: the gradients are
-// read twice, less what the caches keep, and written once.  320 tensors, 57 M elements of bf16 and f32: 60 us + 130 us, 5.3 TB/s of what the two
+// read twice, less what the caches keep, and written once.  320 tensors, 112 M elements of bf16 and f32: 60 us + 130 us, 5.3 TB/s of what the two
 // passes touch; 12 tensors of two small networks: 3.6 us + 3.9 us, launch latency.
 #include <algorithm>
 #include <vector>
@@ -219,7 +219,7 @@ int norm_plan(const marlhip_tensor* t, int32_t count, NormPlan& plan, bool clip)
         total += t[i].n;
         bytes += t[i].n * e;
     }
-    // about 4096 workgroups: enough to fill the chip evenly (2048 took 15 % longer on 57 M elements), few enough sums for every one to add up
+    // about 4096 workgroups: enough to fill the chip evenly (2048 took 15 % longer on 112 M elements), few enough sums for every one to add up
     const int64_t c = (total / NORM_WGS + 4095) / 4096 * 4096;
     plan.chunk = c < 4096 ? 4096 : c;
     plan.stream = bytes > (1ll << 27);

@@ -206,7 +206,7 @@ __device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bia
 // Bound by the vector ALUs: a state of a step is a product, an exponential (two issue slots), a product and two fused multiply-adds, and with the
 // softplus, the gate and the loads a step of 32 channels x 16 states takes 58 instructions.  128 steps x 1024 rows x 128 channels f32: 82 us,
 // 3.3 TB/s, ALUs busy 87 % of the time; the bytes alone would take 64 us.  The inputs of a block are requested a block ahead.
-// CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass: 31 us of the 83 us that
+// CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass: 29 us of the 78 us that
 // 16384 steps x 512 channels bf16 take).
 template <class T, int NL, int NS, bool CARRY>
 __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
@@ -561,7 +561,7 @@ __device__ __forceinline__ void sum_maps(const ScanArgs& a, const float (&red)[W
 // Blocks of K steps from the last to the first: a block's states are recomputed from its record into registers, then its steps run backwards.
 // A workgroup's waves own neighbouring channels of the same rows: they share B and C in LDS and add up their shares of dB and dC there (sums over
 // channels are sums over lanes: pair_sums).  Sums over rows stay in registers until the end.  Bound by the vector ALUs: about 15 instructions a
-// state of a step, a sixth of them for dB and dC.  501 steps x 128 rows x 256 channels bf16: 284 us, ALUs busy 3/4 of the time (two waves a SIMD:
+// state of a step, a sixth of them for dB and dC.  501 steps x 128 rows x 256 channels bf16: 270 us, ALUs busy 82 % of the time (two waves a SIMD:
 // a block's states fill the registers); 26 steps x 1024 rows x 128 channels f32: 73 us.
 template <class T, int NL, int NS>
 __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) {
