@@ -2,10 +2,10 @@
 //
 //   h_t[n] = exp(dt_t A[n]) h_{t-1}[n] + dt_t B_t[n] x_t,   y_t = sum_n C_t[n] h_t[n] + D x_t        for every channel
 //
-// Layout of a wave.  A lane keeps 8 states of one channel in registers, NS = 1, 2 or 4 lanes share a channel (N <= 8, 16, 32): lane =
+// Layout of a wave.  A lane keeps NL = 8 or 4 states of one channel in registers, NS = 1, 2 or 4 lanes share a channel (N <= NL NS): lane =
 // group * CL + channel, CL = 64 / NS channels a wave.  The work of a step that does not depend on the state (loads, softplus, gate, store) is
 // done for NS steps at once, group g taking step s + g; a lane swap then hands every group the step it needs, and another one adds the groups'
-// shares of y.  So NS > 1 costs three swaps a step, keeps 8 / N of the registers and gives NS times the waves, which is what small batches need.
+// shares of y.  So more lanes a channel cost swaps, but take fewer registers and give more waves, which is what small batches need (scan_plan).
 // B and C of a step are the same for a group's channels and come as LDS broadcasts, K steps at a time.
 #include "ssm.h"
 
@@ -401,10 +401,17 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(ScanArgs a) {
     }
 }
 
+// What follows a chunk that starts from h and gives `own` by itself: the decay exp(a sum dt), a = A log2 e, is put on in two factors, since over a
+// whole chunk it may leave the range of a float where its product with the state does not (A > 0 or steps below 0, with an h of 0 for one).
+__device__ __forceinline__ float join_chunk(float a, float sum, float own, float h) {
+    const float r = a * sum, k = fminf(fmaxf(rintf(r), -1000.f), 1000.f);
+    return sum == sum ? ldexpf(exp2_fast(r - k) * h, (int)k) + own : own;
+}
+
 // Joins the chunks of a sequence: carry[j] (what chunk j contributes) becomes what chunk j starts from.  A chunk multiplies what it is given by
 // exp(A sum dt), or drops it at a reset (sum = NaN).  A workgroup takes 64 channels of one state, its 16 waves a run of chunks each; the runs
 // are joined through LDS, so the serial part is nchunk / 16 steps twice and 16 once.  reverse: from the last chunk to the first.
-// Bound by latency: 11 us for 256 chunks of 512 channels x 16 states.
+// Bound by latency: 12 us for 256 chunks of 512 channels x 16 states.
 __global__ __launch_bounds__(1024) void ssm_scan_join_kernel(ScanArgs a, const float* __restrict__ start, int reverse) {
     __shared__ float ls[16][64], lh[16][64];
     const int cbs = (a.d.C + 63) / 64, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -414,25 +421,24 @@ __global__ __launch_bounds__(1024) void ssm_scan_join_kernel(ScanArgs a, const f
     const float A = a.A[((int64_t)a.d.net[row / a.d.B] * a.d.N + n) * a.d.C + c] * LOG2E;
     const int per = (a.nchunk + 15) / 16, lo = w * per, hi = lo + per < a.nchunk ? lo + per : a.nchunk;
     auto at = [&](int k) { return (int64_t)row * a.nchunk + (reverse ? a.nchunk - 1 - k : k); };
-    auto apply = [&](float s, float own, float h) { return s == s ? fmaf(exp2_fast(A * s), h, own) : own; };
     float s = 0.f, h = 0.f;
 #pragma unroll 4
     for (int k = lo; k < hi; ++k) {
         const float sk = a.sums[at(k) * a.d.C + c], own = a.carry[(at(k) * a.d.N + n) * a.d.C + c];
-        h = apply(sk, own, h);
+        h = join_chunk(A, sk, own, h);
         s += sk;
     }
     ls[w][lane] = s;
     lh[w][lane] = h;
     __syncthreads();
     h = start != nullptr ? start[((int64_t)row * a.d.N + n) * a.d.C + c] : 0.f;
-    for (int k = 0; k < w; ++k) h = apply(ls[k][lane], lh[k][lane], h);
+    for (int k = 0; k < w; ++k) h = join_chunk(A, ls[k][lane], lh[k][lane], h);
 #pragma unroll 4
     for (int k = lo; k < hi; ++k) {
         float* q = a.carry + (at(k) * a.d.N + n) * a.d.C + c;
         const float sk = a.sums[at(k) * a.d.C + c], own = *q;
         if (act) *q = h;
-        h = apply(sk, own, h);
+        h = join_chunk(A, sk, own, h);
     }
 }
 
@@ -448,7 +454,7 @@ __global__ __launch_bounds__(256) void ssm_scan_join_few_kernel(ScanArgs a, cons
         const int64_t at = (int64_t)row * a.nchunk + (reverse ? a.nchunk - 1 - k : k);
         const float s = a.sums[at * a.d.C + c], own = a.carry[at * nc + e];
         a.carry[at * nc + e] = h;
-        h = s == s ? fmaf(exp2_fast(A * s), h, own) : own;
+        h = join_chunk(A, s, own, h);
     }
 }
 

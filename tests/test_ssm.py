@@ -156,12 +156,12 @@ def scan_grad_call(v, record):
     return h.ssm_scan_grad(v["dy"], v["x"], v["delta"], v["A"], v["B"], v["C"], record, dh_out=v["dh_out"], **k)
 
 
-def check_scan(v, grads=True):
+def check_scan(v, grads=True, more=0):
     S, B = v["x"].shape[1:3]
     record = h.ssm_scan_record(v["x"], v["A"].shape[1]) if grads else None
     y, hT = scan_call(v, record=record, want_h=True)
     ref = scan_reference(v, grads)
-    n = 4 * S + 128
+    n = 4 * S + 128 + more
     close(y, *ref["y"], n, "y")
     close(hT, *ref["h"], n, "h")
     if not grads:
@@ -208,6 +208,21 @@ def test_scan_networks_shared_between_agents(sharing):
 def test_scan_long_sequences(S, B, C, N):
     check_scan(make_scan(1, S, B, C, N, rate=0.1, reset=False, lengths=False))
     check_scan(make_scan(1, S, B, C, N, dtype=BF16, seed=1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [256, 2048])
+@pytest.mark.parametrize("h0", [0.0, 1e-30])
+def test_scan_of_growing_states(S, h0):
+    """64 steps grow a state by e^96, beyond f32; the states themselves, empty or tiny before, and their gradients stay inside"""
+    v = make_scan(1, S, 1, 20, 4, z=False, bias=False, softplus=False, reset=False, lengths=False)
+    step = torch.arange(S, device="cuda")[None, :, None, None]
+    v["A"] = torch.ones_like(v["A"])
+    v["delta"] = torch.where((step >= 64) & (step < 128), 1.5, 0.0).expand_as(v["x"]).contiguous()
+    v["x"], v["dy"] = torch.where(step >= 110, v["x"], 0.0), torch.where(step <= 70, v["dy"], 0.0)
+    v["h_in"], v["dh_out"] = torch.full_like(v["h_in"], h0), torch.full_like(v["dh_out"], h0)
+    # the exponents add up to 96, each rounded three times (log2 e, A log2 e, the product), once more over a chunk
+    check_scan(v, more=2 * 3 * 96)
 
 
 @pytest.mark.gpu
