@@ -100,6 +100,13 @@ __device__ __forceinline__ float from_groups(const float (&r)[NS]) {
     if constexpr (NS == 4) return half_sum<16>(half_sum<32>(r[0], r[2], 0), half_sum<32>(r[1], r[3], 0), 0);
 }
 
+// waits for loads here: the ones a loop needs from before it are not waited for inside it, where stores would be waited for with them
+template <int N>
+__device__ __forceinline__ void wait_for(float (&r)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) asm volatile("" : "+v"(r[n]));
+}
+
 // ---- K steps of inputs, requested ahead of their use ----------------------------------------------------------------------------------------
 template <class T>
 struct Raw;  // an element as it comes, widened at its use
@@ -181,7 +188,12 @@ __device__ __forceinline__ void store_maps(const Maps<T, NP, NT>& m, float* lb, 
     }
 }
 
-// bit s: an episode starts at step t0 + s
+// bit s: an episode starts at step t0 + s.  Two forms of the load: through a descriptor, without a branch, so that the waits around it stay counted
+// (forwards), and under one, where scalar registers are short (backwards: 261 us, with a descriptor 292)
+__device__ __forceinline__ int load_reset_row(const ScanArgs& a, int b, int t0, int end, int lane) {
+    const auto row = row_rsrc(a.reset + (int64_t)t0 * a.d.B + b, a.reset != nullptr ? ROW_MAX : 0);
+    return __builtin_amdgcn_raw_buffer_load_b8(row, lane % K * a.d.B | behind(t0, lane % K, end), 0, 0);
+}
 __device__ __forceinline__ int load_reset(const ScanArgs& a, int b, int t0, int end, int lane) {
     if (a.reset == nullptr) return 0;
     const int t = t0 + (lane % K);
@@ -208,9 +220,15 @@ __device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bia
 // 3.3 TB/s, ALUs busy 87 % of the time; the bytes alone would take 64 us.  The inputs of a block are requested a block ahead.
 // CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass: 29 us of the 78 us that
 // 16384 steps x 512 channels bf16 take).
-template <class T, int NL, int NS, bool CARRY>
+//
+// The stores of a whole block come together at its end, outside all branches, and the record has a kernel of its own: loads and stores are counted
+// by one counter, and where the number of stores behind the loads for the next block is not known the wait for those loads is one for all stores as
+// well (501 steps x 128 rows x 256 channels bf16 with the record: 120 us, with every wait a counted one 105).
+enum Pass { CARRY_PASS, STEPS_PASS, RECORD_PASS };
+template <class T, int NL, int NS, int PASS>
 __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     constexpr int NP = NS * NL, KG = K / NS;
+    constexpr bool CARRY = PASS == CARRY_PASS;
     __shared__ float lds[4][2][K * NP];
     const int wv = uni(threadIdx.x >> 6);
     const int item = blockIdx.x * 4 + wv;
@@ -223,7 +241,7 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     SeqPtr<T, NS> xs(a.x, q, p, b, first), ds(a.delta, q, p, b, first), zs(a.z, q, p, b, first);
     MapsPtr<T, NP, 64> ms(a, p, b, q.grp, first, threadIdx.x & 63);
     const bool gated = !CARRY && a.z.data != nullptr;
-    const int lane = q.lane;
+    const int lane = q.lane, no_gate = gated ? 0 : OOB;
 
     Raw<T> x[KG], dr[KG], z[KG];
     Maps<T, NP, 64> maps;
@@ -235,13 +253,13 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
                 const int out = behind(t0 + i * NS, q.g, last);
                 xs.load(x[i], i * NS, out);
                 ds.load(dr[i], i * NS, out);
-                if (gated) zs.load(z[i], i * NS, out);
+                if (!CARRY) zs.load(z[i], i * NS, out | no_gate);
             }
             ms.load(maps, t0, last, lane);
         };
         if (t0 + K <= end) load(NO_END);  // a whole block: no offset has to be masked
         else load(end);
-        rs = load_reset(a, b, t0, end, lane);
+        rs = load_reset_row(a, b, t0, end, lane);
         xs.move(K);
         ds.move(K);
         zs.move(K);
@@ -260,11 +278,16 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     const int yoff = q.act ? q.g * (int)(yst * (int64_t)sizeof(T)) + q.cl * (int)sizeof(T) : OOB;
     float *lb = lds[wv][0], *lc = lds[wv][1];
     float total = 0.f;  // CARRY: sum of dt
-    for (int t0 = first; t0 < end; t0 += K) {
+    wait_for(h);
+    float db[2] = {D, bias};
+    wait_for(db);
+    int t0 = first;
+    auto block = [&](auto whole) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole)::v;
         wave_lds_sync();
         store_maps(maps, lb, lc, lane);
         const unsigned fresh = reset_bits(rs);
-        float xv[KG], dt[KG], gate[KG];
+        float xv[KG], dt[KG], gate[KG], yv[KG];  // yv: stored behind both forms of the steps
 #pragma unroll
         for (int i = 0; i < KG; ++i) {
             xv[i] = x[i].get();
@@ -272,19 +295,15 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
             gate[i] = gated ? z[i].get() : 0.f;
         }
         wave_lds_sync();
-        if (t0 + K < end) request(t0 + K);
-        if (!CARRY && a.record != nullptr) store_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, h);
-        // two forms of the same steps: a whole block without resets is straight-line code, so that the maps' LDS reads run ahead of their use;
-        // resets (a select a state) and ends inside a block go through the other one
+        if (WHOLE && t0 + K < end) request(t0 + K);
+        if (PASS == RECORD_PASS) store_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, h);
         auto steps = [&](auto plain) __attribute__((always_inline)) {
             constexpr bool PLAIN = decltype(plain)::v;
 #pragma unroll
             for (int i = 0; i < KG; ++i) {
-                int out = 0;
-                if (!PLAIN) {
+                if (!WHOLE) {
                     if (t0 + i * NS >= end) break;
-                    out = behind(t0 + i * NS, q.g, end);
-                    if (out) dt[i] = 0.f;
+                    if (behind(t0 + i * NS, q.g, end)) dt[i] = 0.f;  // a step behind the end changes nothing: dt = 0, x = 0
                 }
                 float dts[NS], us[NS], ys[NS];
                 to_groups<NS>(dt[i], dts);
@@ -303,16 +322,23 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
                     ys[j] = y;
                 }
                 if (!CARRY) {
-                    float y = fmaf(D, xv[i], from_groups<NS>(ys));
-                    if (gated) y *= gate[i] * sigmoid(gate[i]);
-                    row_store(y, yp + i * NS * yst, ROW_MAX, yoff | out);
+                    yv[i] = fmaf(D, xv[i], from_groups<NS>(ys));
+                    if (gated) yv[i] *= gate[i] * sigmoid(gate[i]);
+                    if (!WHOLE) row_store(yv[i], yp + i * NS * yst, ROW_MAX, yoff | behind(t0 + i * NS, q.g, end));
                 }
             }
         };
-        if (t0 + K <= end && fresh == 0) steps(Idx<1>{});
+        if (WHOLE && fresh == 0) steps(Idx<1>{});
         else steps(Idx<0>{});
+        if (!CARRY && WHOLE)
+#pragma unroll
+            for (int i = 0; i < KG; ++i) row_store(yv[i], yp + i * NS * yst, ROW_MAX, yoff);
         yp += K * yst;
-    }
+    };
+    // three forms of a block: without resets it is straight-line code, so that the maps' LDS reads run ahead of their use; resets are a select a state;
+    // and the last block of a sequence may end inside
+    for (; t0 + K <= end; t0 += K) block(Idx<1>{});
+    if (t0 < end) block(Idx<0>{});
     if (CARRY) {
         store_state(a, q, a.carry + ((int64_t)row * a.nchunk + ch) * N * C, h);
         float r[NS];
@@ -963,13 +989,15 @@ extern "C" int marlhip_ssm_scan(const marlhip_ssm_shape* s, const marlhip_ssm_sc
         a.carry = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.carry);
         a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.sums);
         by_type_and_lanes(s, pl, [&](auto t, auto nl, auto ns) {
-            hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v, true>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v, CARRY_PASS>), grid, dim3(256), 0, st, a);
         });
         MARL_CHECK_LAUNCH("ssm_scan_fwd_kernel");
         if (join(a, a.h_in, 0, st) != 0) return -2;
     }
     by_type_and_lanes(s, pl, [&](auto t, auto nl, auto ns) {
-        hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), decltype(nl)::v, decltype(ns)::v, false>), grid, dim3(256), 0, st, a);
+        constexpr int NL = decltype(nl)::v, NS = decltype(ns)::v;
+        if (a.record != nullptr) hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), NL, NS, RECORD_PASS>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((ssm_scan_fwd_kernel<decltype(t), NL, NS, STEPS_PASS>), grid, dim3(256), 0, st, a);
     });
     MARL_CHECK_LAUNCH("ssm_scan_fwd_kernel");
     return 0;
