@@ -689,13 +689,20 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
             // two forms of the block's steps, as forwards: without resets no step has a branch or a select
             auto steps = [&](auto plain) __attribute__((always_inline)) {
                 constexpr bool PLAIN = decltype(plain)::v;
-                float ea[KEEP ? K : 1][NL];
+                float ea[KEEP ? K : 1][NL], keep_dt[KEEP ? KG : 1][NS], keep_u[KEEP ? KG : 1][NS];
 #pragma unroll
                 for (int i = 0; i < KG; ++i) {
                     const int out = behind(t0 + i * NS, q.g, end);
                     float dts[NS], us[NS], ys[NS];
                     to_groups<NS>(dt[i], dts);
                     to_groups<NS>(dt[i] * x[i], us);
+                    if (KEEP) {
+#pragma unroll
+                        for (int j = 0; j < NS; ++j) {
+                            keep_dt[KEEP ? i : 0][j] = dts[j];
+                            keep_u[KEEP ? i : 0][j] = us[j];
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < NS; ++j) {
                         const int s = i * NS + j;
@@ -727,8 +734,16 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                 for (int i = KG - 1; i >= 0; --i) {
                     if (!KEEP) asm volatile("" : "+v"(dt[i]));
                     float dts[NS], us[NS], gys[NS], gb[NS], ga[NS];
-                    to_groups<NS>(dt[i], dts);
-                    to_groups<NS>(dt[i] * x[i], us);
+                    if (KEEP) {
+#pragma unroll
+                        for (int j = 0; j < NS; ++j) {
+                            dts[j] = keep_dt[KEEP ? i : 0][j];
+                            us[j] = keep_u[KEEP ? i : 0][j];
+                        }
+                    } else {
+                        to_groups<NS>(dt[i], dts);
+                        to_groups<NS>(dt[i] * x[i], us);
+                    }
                     to_groups<NS>(dys[i], gys);
 #pragma unroll
                     for (int j = NS - 1; j >= 0; --j) {
