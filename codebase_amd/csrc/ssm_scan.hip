@@ -7,6 +7,8 @@
 // done for NS steps at once, group g taking step s + g; a lane swap then hands every group the step it needs, and another one adds the groups'
 // shares of y.  So more lanes a channel cost swaps, but take fewer registers and give more waves, which is what small batches need (scan_plan).
 // B and C of a step are the same for a group's channels and come as LDS broadcasts, K steps at a time.
+#include <cfloat>
+
 #include "ssm.h"
 
 using namespace marl;
@@ -59,12 +61,22 @@ struct Lane {
 };
 
 template <int NL, int NS>
-__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<NL, NS>& q, const float* p, float scale, float (&r)[NL]) {
+__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<NL, NS>& q, const float* p, float (&r)[NL]) {
     const int off = q.state_off(a), bytes = p != nullptr ? ROW_MAX : 0;
 #pragma unroll
     for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first, bytes, off | q.no_state(a, n), n * a.d.C * 4);
+}
+// A log2 e of the states.  A rate of -inf empties a state at every step that is there; where a block or chunk has steps that are not, with dt = 0,
+// their product would be NaN, so it becomes the lowest finite value.
+__device__ __forceinline__ float rate(float A) {
+    const float r = A * LOG2E;
+    return r < -FLT_MAX ? -FLT_MAX : r;
+}
+template <int NL, int NS>
+__device__ __forceinline__ void load_rates(const ScanArgs& a, const Lane<NL, NS>& q, int net, float (&A)[NL]) {
+    load_state(a, q, a.A + (int64_t)net * a.d.N * a.d.C, A);
 #pragma unroll
-    for (int n = 0; n < NL; ++n) r[n] *= scale;
+    for (int n = 0; n < NL; ++n) A[n] = rate(A[n]);
 }
 template <int NL, int NS>
 __device__ __forceinline__ void store_state(const ScanArgs& a, const Lane<NL, NS>& q, float* p, const float (&r)[NL]) {
@@ -267,9 +279,9 @@ __global__ __launch_bounds__(256) void ssm_scan_fwd_kernel(ScanArgs a) {
     };
     if (first < end) request(first);
     float A[NL], h[NL];
-    load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
-    if (CARRY) load_state(a, q, (const float*)nullptr, 1.f, h);
-    else load_state(a, q, a.nchunk > 1 ? a.carry + ((int64_t)row * a.nchunk + ch) * N * C : (a.h_in != nullptr ? a.h_in + (int64_t)row * N * C : nullptr), 1.f, h);
+    load_rates(a, q, net, A);
+    if (CARRY) load_state(a, q, (const float*)nullptr, h);
+    else load_state(a, q, a.nchunk > 1 ? a.carry + ((int64_t)row * a.nchunk + ch) * N * C : (a.h_in != nullptr ? a.h_in + (int64_t)row * N * C : nullptr), h);
     const int co = q.chan_off(4);
     const float D = row_load(a.D + (int64_t)net * C + q.first, a.D != nullptr ? ROW_MAX : 0, co);
     const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, co);
@@ -395,7 +407,7 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(ScanArgs a) {
     const float D = row_load(a.D + (int64_t)net * C + q.first, a.D != nullptr ? ROW_MAX : 0, cf);
     const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, cf);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) A[n] *= LOG2E;
+    for (int n = 0; n < NP; ++n) A[n] = rate(A[n]);
     float* lm = lds[wv][0];
     for (int b = slot; b < NB; b += a.slots) {
         const bool fresh = uni(rs) != 0, live = uni(ln) > 0;
@@ -444,7 +456,7 @@ __global__ __launch_bounds__(1024) void ssm_scan_join_kernel(ScanArgs a, const f
     const int n = (blockIdx.x / cbs) % a.d.N, row = blockIdx.x / cbs / a.d.N, c0 = (blockIdx.x % cbs) * 64 + lane;
     const bool act = c0 < a.d.C;
     const int c = act ? c0 : a.d.C - 1;
-    const float A = a.A[((int64_t)a.d.net[row / a.d.B] * a.d.N + n) * a.d.C + c] * LOG2E;
+    const float A = rate(a.A[((int64_t)a.d.net[row / a.d.B] * a.d.N + n) * a.d.C + c]);
     const int per = (a.nchunk + 15) / 16, lo = w * per, hi = lo + per < a.nchunk ? lo + per : a.nchunk;
     auto at = [&](int k) { return (int64_t)row * a.nchunk + (reverse ? a.nchunk - 1 - k : k); };
     float s = 0.f, h = 0.f;
@@ -473,7 +485,7 @@ __global__ __launch_bounds__(256) void ssm_scan_join_few_kernel(ScanArgs a, cons
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, nc = (int64_t)a.d.N * a.d.C;
     if (i >= (int64_t)a.d.P * a.d.B * nc) return;
     const int row = (int)(i / nc), e = (int)(i % nc), c = e % a.d.C;
-    const float A = a.A[a.d.net[row / a.d.B] * nc + e] * LOG2E;
+    const float A = rate(a.A[a.d.net[row / a.d.B] * nc + e]);
     float h = start != nullptr ? start[i] : 0.f;
 #pragma unroll 4
     for (int k = 0; k < a.nchunk; ++k) {
@@ -504,8 +516,8 @@ __global__ __launch_bounds__(256) void ssm_scan_bwd_carry_kernel(ScanArgs a) {
     MapsPtr<T, NP, 64> ms(a, p, b, q.grp, tl, threadIdx.x & 63);
     const bool gated = a.z.data != nullptr;
     float A[NL], dh[NL];
-    load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
-    load_state(a, q, (const float*)nullptr, 1.f, dh);
+    load_rates(a, q, net, A);
+    load_state(a, q, (const float*)nullptr, dh);
     const int co = q.chan_off(4);
     const float bias = row_load(a.bias + (int64_t)net * C + q.first, a.bias != nullptr ? ROW_MAX : 0, co);
     float *lb = lds[wv][0], *lc = lds[wv][1];
@@ -612,7 +624,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
     if (kblk >= a.nblk) q.act = false;
     const int N = a.d.N, C = a.d.C, S = a.d.S, NB = a.d.B, net = a.d.net[p], lane = q.lane;
     float A[NL], dA[NL];
-    load_state(a, q, a.A + (int64_t)net * N * C, LOG2E, A);
+    load_rates(a, q, net, A);
 #pragma unroll
     for (int n = 0; n < NL; ++n) dA[n] = 0.f;
     const int co = q.chan_off(4);
@@ -633,7 +645,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
         const int64_t pm = om + (int64_t)run * a.d.P * S * NB * a.d.G * N;
         T *dxp = static_cast<T*>(a.dx) + o, *ddp = static_cast<T*>(a.ddelta) + o, *dzp = static_cast<T*>(a.dz) + o;
         float dh[NL];
-        load_state(a, q, a.nchunk > 1 ? a.carry + ((int64_t)row * a.nchunk + ch) * N * C : (a.dh_out != nullptr ? a.dh_out + (int64_t)row * N * C : nullptr), 1.f, dh);
+        load_state(a, q, a.nchunk > 1 ? a.carry + ((int64_t)row * a.nchunk + ch) * N * C : (a.dh_out != nullptr ? a.dh_out + (int64_t)row * N * C : nullptr), dh);
         for (int t = last - 1; t >= end && t >= first; --t) {  // behind the end
             const int off = q.g == 0 ? q.chan_off(sizeof(T)) : OOB;
             row_store(0.f, dxp + t * yst, ROW_MAX, off);
@@ -655,7 +667,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                 if (gated) zs.load(zr[i], i * NS, out);
             }
             rs = load_reset(a, b, t0, end, lane);
-            load_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, 1.f, hb);
+            load_state(a, q, a.record + ((int64_t)row * a.nck + t0 / K) * N * C, hb);
             if (wv == 0) ms.load(maps, t0, end, lane);
             xs.move(-K);
             ds.move(-K);

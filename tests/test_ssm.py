@@ -226,6 +226,26 @@ def test_scan_of_growing_states(S, h0):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 1, 3, 20, 4), (1, 13, 4, 40, 16), (1, 21, 3, 20, 32), (1, 300, 2, 20, 8)], ids=lambda s: "x".join(map(str, s)))
+def test_scan_of_states_that_forget_at_once(shape):
+    """a rate of -inf: the decay of every step is 0, as with one so low that it rounds to 0, and steps that are not there change nothing"""
+    v = make_scan(*shape, seed=5)
+    P, S, B, C, N = shape
+    v["lengths"] = torch.randint(0, S + 1, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    runs = []
+    for low in (-1e30, float("-inf")):
+        w = dict(v)
+        w["A"] = v["A"].clone()
+        w["A"][:, ::2] = low
+        rec = h.ssm_scan_record(w["x"], N)
+        y, hT = scan_call(w, record=rec, want_h=True)
+        g = scan_grad_call(w, rec)
+        runs.append((y, hT, scan_call(w), *g))
+    for a, b in zip(*runs):
+        assert bool(torch.isfinite(b).all()) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_scan_many_rows():
     """more rows than waves: a wave takes several, and its sums over them stay in registers"""
     check_scan(make_scan(2, 4, 5000, 16, 4, seed=3))
