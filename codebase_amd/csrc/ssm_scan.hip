@@ -228,9 +228,9 @@ __device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bia
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
 // Bound by the vector ALUs: a state of a step is a product, an exponential (two issue slots), a product and two fused multiply-adds, and with the
-// softplus, the gate and the loads a step of 32 channels x 16 states takes 58 instructions.  128 steps x 1024 rows x 128 channels f32: 82 us,
-// 3.3 TB/s, ALUs busy 87 % of the time; the bytes alone would take 64 us.  The inputs of a block are requested a block ahead.
-// CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass: 29 us of the 78 us that
+// softplus, the gate and the loads a step of 32 channels x 16 states takes 58 instructions.  128 steps x 1024 rows x 128 channels f32: 80 us,
+// 3.8 TB/s; the bytes alone would take 64 us.  The inputs of a block are requested a block ahead.
+// CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass: 29 us of the 77 us that
 // 16384 steps x 512 channels bf16 take).
 //
 // The stores of a whole block come together at its end, outside all branches, and the record has a kernel of its own: loads and stores are counted
@@ -605,7 +605,7 @@ __device__ __forceinline__ void sum_maps(const ScanArgs& a, const float (&red)[W
 // Blocks of K steps from the last to the first: a block's states are recomputed from its record into registers, then its steps run backwards.
 // A workgroup's waves own neighbouring channels of the same rows: they share B and C in LDS and add up their shares of dB and dC there (sums over
 // channels are sums over lanes: pair_sums).  Sums over rows stay in registers until the end.  Bound by the vector ALUs: about 15 instructions a
-// state of a step, a sixth of them for dB and dC.  501 steps x 128 rows x 256 channels bf16: 270 us, ALUs busy 82 % of the time (two waves a SIMD:
+// state of a step, a sixth of them for dB and dC.  501 steps x 128 rows x 256 channels bf16: 260 us, ALUs busy 82 % of the time (two waves a SIMD:
 // a block's states fill the registers); 26 steps x 1024 rows x 128 channels f32: 73 us.
 template <class T, int NL, int NS>
 __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) {
@@ -845,9 +845,10 @@ struct ScanPlan {
 // How a call is split.  A row of N states a channel takes N / 8 x C / 64 waves with 8 states a lane; the chip has 1024 SIMDs and wants about
 // four waves on each.
 //   <= 512 waves and long enough: the sequences are cut into chunks of at least 64 steps for 4096 waves.  That costs a first pass of about 0.8
-//     of the second (16384 steps x 512 channels bf16: 12300 us in one piece, 33 + 12 + 43 us in 256 chunks).
+//     of the second (16384 steps x 512 channels bf16: 12300 us in one piece, 29 + 12 + 36 us in 256 chunks).
 //   <= 1024 waves otherwise: 4 states a lane, twice the waves for a sixth more instructions (501 steps x 128 rows x 256 channels bf16: forwards
-//     146 -> 120 us; cut into 4 chunks 158.  Backwards 582 -> 388; cut 376.  With 2048 waves 8 a lane are better: 74 against 80 us).
+//     113 -> 97 us; cut into 4 chunks 141.  Backwards 486 -> 262; cut 330.  With 2048 waves 8 a lane are better: 128 steps x 256 rows x 256
+//     channels, forwards with the record 51 against 57 us, backwards 144 against 147).
 ScanPlan scan_plan(const marlhip_ssm_shape* s) {
     constexpr int64_t CUT_WAVES = 512, FEW_WAVES = 1024, WANT_WAVES = 4096;
     constexpr int CUT_STEPS = 64;
