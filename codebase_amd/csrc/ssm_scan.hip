@@ -718,18 +718,16 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
 #pragma unroll
                     for (int j = 0; j < NS; ++j) {
                         const int s = i * NS + j;
-                        // a reset empties the state through the decay, e^-inf = 0; what is not finite has to go by hand
-                        const bool re = !PLAIN && (fresh >> s & 1);
-                        const float fr = re ? -INFINITY : 0.f;
-                        int lre = re;
+                        // a reset: the step starts from 0.  hs[s] stays what it is, the state after the step before, whose dC is made of it
+                        int lre = !PLAIN && (fresh >> s & 1);
                         if (!PLAIN) asm volatile("" : "+v"(lre));  // a lane's own flag: a select a state, where the compiler would branch for each
                         float y = 0.f;
 #pragma unroll
                         for (int n = 0; n < NL; ++n) {
-                            if (!PLAIN) hs[s][n] = ((lre != 0) & !(fabsf(hs[s][n]) < INFINITY)) ? 0.f : hs[s][n];
-                            const float ex = exp2_fast(PLAIN ? dts[j] * A[n] : fmaf(dts[j], A[n], fr));
+                            const float ex = exp2_fast(dts[j] * A[n]);
                             if (KEEP) ea[KEEP ? s : 0][n] = ex;
-                            hs[s + 1][n] = fmaf(ex, hs[s][n], us[j] * lb[s * NP + q.n0 + n]);
+                            const float ub = us[j] * lb[s * NP + q.n0 + n], hn = fmaf(ex, hs[s][n], ub);
+                            hs[s + 1][n] = lre == 0 ? hn : ub;
                             y = fmaf(hs[s + 1][n], lc[s * NP + q.n0 + n], y);
                         }
                         ys[j] = y;
@@ -760,8 +758,7 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
 #pragma unroll
                     for (int j = NS - 1; j >= 0; --j) {
                         const int s = i * NS + j;
-                        const bool re = !PLAIN && (fresh >> s & 1);
-                        const float fr = re ? -INFINITY : 0.f;
+                        const bool re = !PLAIN && (fresh >> s & 1);  // nothing goes from the step to the state before it
                         float sb = 0.f, sa = 0.f;
                         auto state = [&](auto idx, float& vb, float& vc) __attribute__((always_inline)) {
                             constexpr int n = decltype(idx)::v;
@@ -769,11 +766,14 @@ __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) 
                             const float gn = fmaf(gys[j], lc[s * NP + q.n0 + n], dh[n]);
                             vb = gn * us[j];             // dB
                             sb = fmaf(gn, lb[s * NP + q.n0 + n], sb);
-                            dh[n] = gn * (KEEP ? ea[KEEP ? s : 0][n] : exp2_fast(PLAIN ? dts[j] * A[n] : fmaf(dts[j], A[n], fr)));
-                            const float w = dh[n] * hs[s][n];
+                            dh[n] = gn * (KEEP ? ea[KEEP ? s : 0][n] : exp2_fast(dts[j] * A[n]));
+                            float w = dh[n] * hs[s][n];
+                            if (!PLAIN) {
+                                w = re ? 0.f : w;
+                                dh[n] = re ? 0.f : dh[n];
+                            }
                             sa = fmaf(w, A[n], sa);
                             dA[n] = fmaf(w, dts[j], dA[n]);
-                            if (!PLAIN) dh[n] = re ? 0.f : dh[n];
                         };
                         const float sum = pair_sums<NL, TOP>(state, lane);
                         gb[j] = sb;
