@@ -440,10 +440,11 @@ __global__ __launch_bounds__(256) void ssm_scan_step_kernel(ScanArgs a) {
 }
 
 // What follows a chunk that starts from h and gives `own` by itself: the decay exp(a sum dt), a = A log2 e, is put on in two factors, since over a
-// whole chunk it may leave the range of a float where its product with the state does not (A > 0 or steps below 0, with an h of 0 for one).
+// whole chunk, or a run of them, it may leave the range of a float where its product with the state does not (A > 0 or steps below 0).  A state of 0
+// stays 0 even where the decay is infinite.
 __device__ __forceinline__ float join_chunk(float a, float sum, float own, float h) {
     const float r = a * sum, k = fminf(fmaxf(rintf(r), -1000.f), 1000.f);
-    return sum == sum ? ldexpf(exp2_fast(r - k) * h, (int)k) + own : own;
+    return sum == sum && h != 0.f ? ldexpf(exp2_fast(r - k) * h, (int)k) + own : own;
 }
 
 // Joins the chunks of a sequence: carry[j] (what chunk j contributes) becomes what chunk j starts from.  A chunk multiplies what it is given by
