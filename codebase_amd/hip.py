@@ -1406,12 +1406,15 @@ def _ssm_shape(what, x, state, groups, sharing):
     if code is None:
         raise ValueError(f"{what}: {x.dtype} is not supported (float32, bfloat16, float16)")
     P, S, B, C = x.shape
-    if sharing is None:
-        return _SHAPE_PACK(P, S, B, C, state, groups, code, 0, *_NO_NETS), P, x.get_device()
-    if len(sharing) != P or P > 16:
-        raise ValueError(f"{what}: sharing indices: one per agent, at most 16 agents")
-    M = max(sharing) + 1
-    return _SHAPE_PACK(P, S, B, C, state, groups, code, M, *sharing, *_NO_NETS[P:]), M, x.get_device()
+    try:
+        if sharing is None:
+            return _SHAPE_PACK(P, S, B, C, state, groups, code, 0, *_NO_NETS), P, x.get_device()
+        if len(sharing) != P or not 1 <= P <= 16:
+            raise ValueError(f"{what}: sharing indices: one per agent, at most 16 agents")
+        M = max(sharing) + 1
+        return _SHAPE_PACK(P, S, B, C, state, groups, code, M, *sharing, *_NO_NETS[P:]), M, x.get_device()
+    except struct.error:  # the C struct holds 32-bit integers
+        raise ValueError(f"{what}: shape {tuple(x.shape)}, {state} states or taps, {groups} groups, sharing {sharing}: not 32-bit integers") from None
 
 
 _NO_NETS = (0,) * 16

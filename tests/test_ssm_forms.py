@@ -54,3 +54,12 @@ def test_empty_states_in_sequences_that_grow(S):
     w = dict(v, x=torch.zeros_like(v["x"]), dy=torch.where(early, v["dy"], 0.0), delta=torch.where(early, 0.01, grow))
     _, _, g = check_scan(w)
     assert g.x.any()
+
+
+def test_sizes_beyond_the_c_structs_are_refused():
+    x, w = torch.zeros(2, 1, 1, 4), torch.zeros(2, 4, 4)
+    for call in (lambda: h.ssm_conv(x[:1].expand(1, 1, 2**31, 4), w[:1]), lambda: h.ssm_scan_record(x, 2**31), lambda: h.ssm_conv(x, w, sharing=(0, 1.0))):
+        with pytest.raises(ValueError, match="not 32-bit integers"):
+            call()
+    with pytest.raises(ValueError, match="one per agent"):
+        h.ssm_conv(x[:0], w, sharing=())
