@@ -131,6 +131,23 @@ def test_two_streams_at_once():
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.gpu
+def test_a_tensor_of_several_pieces():
+    """more elements than one entry of the kernel's table holds (2^30), the last ones alone in a second"""
+    n = 2**30 + 4099
+    t = torch.zeros(n, dtype=torch.float16, device="cuda")
+    t[::1021], t[2**30 - 3:] = 0.5, 2.0
+    small = torch.full((77,), 3.0, device="cuda")
+    ones = (n + 1020) // 1021 - len(range(0, n, 1021)[(2**30 - 3 + 1020) // 1021:])
+    norm = math.sqrt(0.25 * ones + 4.0 * (4099 + 3) + 9.0 * 77)
+    got = h.clip_grad_norm([t, small], 1.0)
+    assert abs(got.item() - norm) <= 2 * U * norm
+    want = torch.zeros(n, dtype=torch.float16, device="cuda")
+    want[::1021], want[2**30 - 3:] = t[0].item(), t[-1].item()
+    assert torch.equal(t, want)
+    check_clipped([t[:1], t[-1:], small], [torch.tensor([c / (norm + 1e-6)], dtype=torch.float64, device="cuda") for c in (0.5, 2.0, 3.0)])
+
+
 # ---- refusals (no device is touched) -------------------------------------------------------------------------------------------------
 def test_refusals():
     t = torch.zeros(4, 6)

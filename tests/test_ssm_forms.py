@@ -4,11 +4,110 @@ import pytest
 import torch
 
 from codebase_amd import hip as h
-from tests.test_ssm import check_scan, make_scan, scan_call, scan_grad_call
+from tests.test_ssm import BF16, F16, F32, HALF, TINY, U, check_conv, check_scan, conv_call, live_and_fresh, make_conv, make_scan, scan_call, scan_grad_call
+
+TYPES = pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
 
 
 def name_of(shape):
     return "x".join(map(str, shape))
+
+
+# P, S, B, C, N, G.  More than 1024 waves of 8 states a lane take 8, on one lane up to 8 states, on two up to 16; fewer take 4
+WHOLE = [(3, 11, 200, 70, 8, 1), (2, 13, 300, 100, 7, 2), (2, 9, 300, 40, 16, 1), (1, 26, 600, 66, 10, 2), (1, 10, 150, 288, 16, 1)]
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("shape", WHOLE, ids=name_of)
+def test_many_whole_rows(shape, dtype):
+    v = make_scan(*shape, dtype=dtype, seed=sum(shape), sharing=(0,) * shape[0])
+    check_scan(v)
+    check_scan(v, grads=False)
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("shape", [(2, 2, 5, 64, 16, 1), (1, 7, 3, 63, 4, 1), (2, 17, 2, 96, 24, 3), (1, 19, 2, 200, 32, 1), (1, 33, 2, 130, 9, 2)], ids=name_of)
+def test_forward_without_a_record(shape, dtype):
+    check_scan(make_scan(*shape, dtype=dtype, seed=sum(shape)), grads=False)
+
+
+@pytest.mark.gpu
+@TYPES
+# with 8192 waves for them all, a wave takes several rows
+@pytest.mark.parametrize("shape", [(2, 1, 5000, 20, 4, 1), (1, 1, 3000, 130, 16, 1), (2, 1, 2100, 66, 20, 2), (1, 1, 9000, 40, 32, 1), (3, 1, 7, 65, 5, 1)], ids=name_of)
+def test_single_steps(shape, dtype):
+    check_scan(make_scan(*shape, dtype=dtype, seed=sum(shape)), grads=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("absent", ["z", "D", "bias", "carry", "reset", "lengths", "softplus"])
+def test_single_steps_without(absent):
+    v = make_scan(3, 1, 40, 70, 12, G=2, sharing=(1, 0, 1), **{absent: False})
+    y, _, _ = check_scan(v, grads=False)
+    assert torch.equal(scan_call(v), y)  # the state not asked for
+
+
+def rounding_reference(v):
+    """y and h in 64 bits, each with the sum of what its roundings can amount to in units of u: a step's decay carries the roundings made so far
+    on, so that those of a long sequence fade as its states do.
+
+    dt: raw = delta + bias is off by u |raw|, which e^-|raw| turns into as much of dt; the exponent's product with log2 e doubles that; exponential, sum,
+    logarithm, correction and final sum: 8 more.  A decay: three roundings of the exponent dt A log2 e next to dt's own, the exponential's 2, the product's and the sum's."""
+    x, S = v["x"].double(), v["x"].shape[1]
+    P, _, B, C = x.shape
+    N, G = v["A"].shape[1], v["B"].shape[3]
+    A, D, bias = v["A"].double(), v["D"].double(), v["delta_bias"].double()
+    live, fresh = live_and_fresh(S, B, v["reset"], v["lengths"], x.device)
+    hc = v["h_in"].double()
+    mag, err, ys, es = hc.abs(), torch.zeros_like(hc), [], []
+    for t in range(S):
+        lv, fr = live[t][None, :, None, None], fresh[t][None, :, None, None]
+        raw = v["delta"][:, t].double() + bias[:, None]
+        dt, ddt = torch.nn.functional.softplus(raw, threshold=100.0), 8 + 3 * raw.abs()
+        Bt, Ct = (v[k][:, t].double().transpose(-1, -2).repeat_interleave(C // G, -1) for k in ("B", "C"))
+        power = dt[:, :, None] * A[:, None]
+        decay, u = torch.exp(power), (dt * x[:, t])[:, :, None] * Bt
+        hp, mp, ep = (torch.where(fr, 0.0, q) for q in (hc, mag, err))
+        mn = decay * mp + u.abs()
+        en = decay * (ep + (4 + power.abs() * (3 + ddt[:, :, None])) * mp) + (3 + ddt[:, :, None]) * u.abs() + mn
+        hn = decay * hp + u
+        y, ym = (Ct * hn).sum(2) + D[:, None] * x[:, t], (Ct.abs() * mn).sum(2) + (D[:, None] * x[:, t]).abs()
+        ye = (Ct.abs() * en).sum(2) + (N + 2) * ym
+        if v["z"] is not None:
+            z = v["z"][:, t].double()
+            gate = z * torch.sigmoid(z)
+            y, ym, ye = y * gate, ym * gate.abs(), ye * gate.abs() + (8 + 2 * z.abs()) * ym * gate.abs()
+        ys.append(torch.where(lv[..., 0], y, 0.0))
+        es.append(torch.where(lv[..., 0], torch.stack([ym, ye])[:, :, :, :], 0.0))
+        hc, mag, err = (torch.where(lv, n, q) for n, q in ((hn, hc), (mn, mag), (en, err)))
+    return torch.stack(ys, 1), torch.stack(es, 2), hc, torch.stack([mag, err])
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("rate", [0.01, 1.0])
+# 17, 18 and 6 chunks; 64 steps and more a chunk, the last ones short or behind the end
+@pytest.mark.parametrize("shape", [(2, 1200, 3, 70, 16, 1), (1, 1153, 4, 130, 9, 2), (1, 400, 5, 72, 24, 1)], ids=name_of)
+def test_long_rows_in_chunks(shape, rate, dtype):
+    P, S, B, C, N, G = shape
+    v = make_scan(*shape, dtype=dtype, seed=S, rate=rate)
+    # chunks with and without a reset inside, at their first and last steps, and rows that end in different chunks
+    gen = torch.Generator().manual_seed(1)
+    v["reset"] = (torch.rand(S, B, generator=gen) < 0.004).to(torch.uint8)
+    v["reset"][72], v["reset"][143, 0], v["reset"][0, 1] = 1, 1, 1
+    v["reset"] = v["reset"].cuda()
+    v["lengths"] = torch.tensor([S, 0, S // 2, S - 3, 71][:B], dtype=torch.int32, device="cuda")
+    # a chunk's decay: sum of dt over up to 72 steps, each partial sum rounded; x e^-x <= 0.37 times 72 + 8 is below 32 a chunk, and a state
+    # passes at most 18 of them
+    y, hT, _ = check_scan(v)
+    yr, (ym, ye), hr, (hm, he) = rounding_reference(v)
+    for got, (ref, mag, err) in ((y, (yr, ym, ye)), (hT, (hr, hm, he))):
+        bound = U * (err + 32 * 18 * mag)
+        bound = bound + HALF[got.dtype] * (ref.abs() + bound) + TINY[got.dtype]
+        assert bool(((got.double() - ref).abs() <= bound).all())
+    assert torch.equal(scan_call(v), y)
 
 
 @pytest.mark.gpu
@@ -54,6 +153,42 @@ def test_empty_states_in_sequences_that_grow(S):
     w = dict(v, x=torch.zeros_like(v["x"]), dy=torch.where(early, v["dy"], 0.0), delta=torch.where(early, 0.01, grow))
     _, _, g = check_scan(w)
     assert g.x.any()
+
+
+# P, S, B, C, W: stretches of 16 and of 32 steps, 8 channels a thread and one
+CONV = [(1, 40, 6600, 64, 4), (2, 70, 1900, 128, 3), (1, 66, 2100, 255, 4)]
+
+
+@pytest.mark.gpu
+@TYPES
+@pytest.mark.parametrize("shape", CONV, ids=name_of)
+def test_conv_longer_stretches(shape, dtype):
+    v = make_conv(*shape, dtype=dtype, seed=sum(shape))
+    y, end, _ = check_conv(v)
+    state = v["state"].clone()
+    assert torch.equal(conv_call(v, state=state, state_out=state), y) and torch.equal(state, end)
+
+
+@pytest.mark.gpu
+@TYPES
+# more rows and stretches than the workgroups of a channel tile take at once
+@pytest.mark.parametrize("shape", [(1, 9, 2100, 512, 4), (1, 9, 2100, 65, 2), (2, 17, 700, 260, 5), (4, 1, 2100, 512, 4)], ids=name_of)
+def test_conv_gradient_of_many_rows(shape, dtype):
+    check_conv(make_conv(*shape, dtype=dtype, seed=sum(shape)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad", [0, 1])
+def test_conv_offsets_beyond_32_bits(pad):
+    """steps 2^28 elements (2^29 bytes) apart: the last one starts 5.5 GiB into the buffer"""
+    P, S, B, C, W = 1, 12, 2, 64, 4
+    v = make_conv(P, S, B, C, W, dtype=BF16)
+    for k in ("x", "dy"):
+        big = torch.empty(11 * 2**28 + B * C + pad, dtype=BF16, device="cuda")
+        far = big.as_strided((P, S, B, C), (0, 2**28, C, 1), pad)
+        far.copy_(v[k])
+        v[k] = far
+    check_conv(v)
 
 
 def test_sizes_beyond_the_c_structs_are_refused():
