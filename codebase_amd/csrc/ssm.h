@@ -130,8 +130,9 @@ __device__ __forceinline__ float half_sum(float lo, float hi, int lane) {
 }
 
 // Sums of NL pairs over the TOP * 2 lanes of a group, formed as the pairs appear: f(n, b, c) gives (b_n, c_n).  The pairs merge as soon as two
-// exist - about 2 instructions a value, where a butterfly each would take 2 log2(lanes) - and need a handful of registers.  gfx950's lane
-// swaps exchange halves of two registers in one instruction; inside a row of 16 lanes the partners are mirrors (DPP).  Lane bit TOP tells b
+// exist - 2 to 3 instructions a value, where a butterfly each would take 2 log2(lanes) - and need a handful of registers.  gfx950's lane
+// swaps exchange halves of two registers in one instruction, so that a merge takes 2; inside a row of 16 lanes the partners are mirrors (DPP),
+// and it takes 3, two selects and an addition (every merge where four lanes share a channel: TOP = 8).  Lane bit TOP tells b
 // from c, the log2(NL) below it are n; lanes that differ in lower bits only hold the same sum.
 template <int NL, int TOP, int LVL, int I, class F>
 __device__ __forceinline__ float pair_tree(F& f, int lane) {

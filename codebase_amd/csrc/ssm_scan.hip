@@ -67,7 +67,7 @@ __device__ __forceinline__ void load_state(const ScanArgs& a, const Lane<NL, NS>
     for (int n = 0; n < NL; ++n) r[n] = row_load(p + q.first, bytes, off | q.no_state(a, n), n * a.d.C * 4);
 }
 // A log2 e of the states.  A rate of -inf empties a state at every step that is there; where a block or chunk has steps that are not, with dt = 0,
-// their product would be NaN, so it becomes the lowest finite value.
+// their product would be NaN, so it becomes the lowest finite value (which empties a state unless dt is below 2^-120).
 __device__ __forceinline__ float rate(float A) {
     const float r = A * LOG2E;
     return r < -FLT_MAX ? -FLT_MAX : r;
@@ -228,7 +228,7 @@ __device__ __forceinline__ float step_size(const ScanArgs& a, float d, float bia
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
 // Bound by the vector ALUs: a state of a step is a product, an exponential (two issue slots), a product and two fused multiply-adds, and with the
-// softplus, the gate and the loads a step of 32 channels x 16 states takes 58 instructions.  128 steps x 1024 rows x 128 channels f32: 80 us,
+// softplus, the gate and the loads a step of 32 channels x 16 states takes 58 instructions.  128 steps x 1024 rows x 128 channels f32: 79 us,
 // 3.8 TB/s; the bytes alone would take 64 us.  The inputs of a block are requested a block ahead.
 // CARRY: only the state a chunk contributes and its sum of dt are formed (sequences split over their length, first pass: 29 us of the 77 us that
 // 16384 steps x 512 channels bf16 take).
@@ -450,7 +450,7 @@ __device__ __forceinline__ float join_chunk(float a, float sum, float own, float
 // Joins the chunks of a sequence: carry[j] (what chunk j contributes) becomes what chunk j starts from.  A chunk multiplies what it is given by
 // exp(A sum dt), or drops it at a reset (sum = NaN).  A workgroup takes 64 channels of one state, its 16 waves a run of chunks each; the runs
 // are joined through LDS, so the serial part is nchunk / 16 steps twice and 16 once.  reverse: from the last chunk to the first.
-// Bound by latency: 12 us for 256 chunks of 512 channels x 16 states.
+// Bound by latency: 12.6 us for 256 chunks of 512 channels x 16 states, 128 workgroups on half of the compute units.
 __global__ __launch_bounds__(1024) void ssm_scan_join_kernel(ScanArgs a, const float* __restrict__ start, int reverse) {
     __shared__ float ls[16][64], lh[16][64];
     const int cbs = (a.d.C + 63) / 64, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -605,9 +605,11 @@ __device__ __forceinline__ void sum_maps(const ScanArgs& a, const float (&red)[W
 
 // Blocks of K steps from the last to the first: a block's states are recomputed from its record into registers, then its steps run backwards.
 // A workgroup's waves own neighbouring channels of the same rows: they share B and C in LDS and add up their shares of dB and dC there (sums over
-// channels are sums over lanes: pair_sums).  Sums over rows stay in registers until the end.  Bound by the vector ALUs: about 15 instructions a
-// state of a step, a sixth of them for dB and dC.  501 steps x 128 rows x 256 channels bf16: 260 us, ALUs busy 82 % of the time (two waves a SIMD:
-// a block's states fill the registers); 26 steps x 1024 rows x 128 channels f32: 73 us.
+// channels are sums over lanes: pair_sums).  Sums over rows stay in registers until the end.  Bound by the vector ALUs: 501 steps x 128 rows x 256
+// channels bf16 take 260 us with 29 instructions a state of a step (counted), the ALUs busy 86 % of the time that the compute units are (two waves a
+// SIMD: a block's states fill the registers).  About 7 of the 29 recompute the states, 15 walk back over them - a third of those merge lanes for dB
+// and dC - and the rest are inputs, sums over waves, stores and scalars that spill.  26 steps x 1024 rows x 128 channels f32: 73 us; its last block
+// of 8 steps has 2 that are there, and all 8 are worked on.
 template <class T, int NL, int NS>
 __global__ __launch_bounds__(64 * WMAX, 2) void ssm_scan_bwd_kernel(ScanArgs a) {
     constexpr int NP = NS * NL, KG = K / NS, TOP = 32 / NS;
@@ -846,7 +848,7 @@ struct ScanPlan {
 // How a call is split.  A row of N states a channel takes N / 8 x C / 64 waves with 8 states a lane; the chip has 1024 SIMDs and wants about
 // four waves on each.
 //   <= 512 waves and long enough: the sequences are cut into chunks of at least 64 steps for 4096 waves.  That costs a first pass of about 0.8
-//     of the second (16384 steps x 512 channels bf16: 12300 us in one piece, 29 + 12 + 36 us in 256 chunks).
+//     of the second (16384 steps x 512 channels bf16: 12300 us in one piece, 29 + 13 + 36 us in 256 chunks).
 //   <= 1024 waves otherwise: 4 states a lane, twice the waves for a sixth more instructions (501 steps x 128 rows x 256 channels bf16: forwards
 //     113 -> 97 us; cut into 4 chunks 141.  Backwards 486 -> 262; cut 330.  With 2048 waves 8 a lane are better: 128 steps x 256 rows x 256
 //     channels, forwards with the record 51 against 57 us, backwards 144 against 147).

@@ -1492,7 +1492,8 @@ def ssm_conv(x, weight, bias=None, silu=True, sharing=None, state=None, want_sta
     x [P][S][B][C] (S = 1: one acting step), weight f32 [M][W][C] (W <= 8), bias f32 [M][C] or None; `sharing` maps agents to the M networks
     (None: one each).  `state` [P][B][W-1][C]: the inputs before step 0 (None: zeros); `want_state` returns the ones after the last step, or
     `state_out` receives them (`state` itself: updated in place).  `reset` u8/bool [S][B]: an episode starts at this step, nothing before it
-    is seen; `lengths` i32 [B]: steps of a row, those behind are not read and give 0.  -> y, or (y, state_out)"""
+    is seen; `lengths` i32 [B]: steps of a row, what stands behind them does not matter and gives 0.  Outputs share no memory with other arguments.
+    -> y, or (y, state_out)"""
     shape, dev, xs, w, b, st, rs, ln, window = _conv_args("ssm_conv", x, weight, bias, sharing, state, reset, lengths)
     so = _dense("ssm_conv", "state_out", state_out, window, x.dtype, dev)
     _in_place_or_apart("ssm_conv", "state_out", state_out, state)
@@ -1507,8 +1508,8 @@ def ssm_conv(x, weight, bias=None, silu=True, sharing=None, state=None, want_sta
 
 
 def ssm_conv_grad(dy, x, weight, bias=None, silu=True, sharing=None, state=None, reset=None, lengths=None, dstate_out=None):
-    """gradients of ssm_conv for the same arguments: dy [P][S][B][C] at y and (optional) dstate_out [P][B][W-1][C] at state_out ->
-    SsmConvGrad(x, weight, bias, state); bias / state are None where the argument is"""
+    """gradients of ssm_conv for the same arguments (`state` as it was before an update in place): dy [P][S][B][C] at y and (optional) dstate_out
+    [P][B][W-1][C] at state_out -> SsmConvGrad(x, weight, bias, state); bias / state are None where the argument is"""
     shape, dev, xs, w, b, st, rs, ln, window = _conv_args("ssm_conv_grad", x, weight, bias, sharing, state, reset, lengths)
     if dy is None:
         raise ValueError("ssm_conv_grad: dy is not a tensor")

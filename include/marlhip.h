@@ -843,17 +843,20 @@ int marlhip_qmix_update_n(const marlhip_qmix_learner* L, int32_t n_updates, int3
  * next to the GRU sequences above (marlhip_gru_forward: same [agent][step][row] layout, same carried state between calls).  They have no
  * counterpart in the reference, whose recurrent networks are GRUs (marlbase/utils/models.py:74-90).
  *
- * Sequences: element (p, t, b, c) at data + p * agent_stride + t * step_stride + b * row_stride + c, strides in ELEMENTS, any value
- * (slices of wider projections, broadcast strides 0 for inputs); data == NULL: absent.  Outputs are contiguous [P][S][B][C].
+ * Sequences: element (p, t, b, c) at data + p * agent_stride + t * step_stride + b * row_stride + c, strides in ELEMENTS (slices of wider
+ * projections, broadcast strides 0 for inputs); data == NULL: absent.  Where a scan has more than one step, its step strides are 0..2^29 bytes,
+ * those of B and C 0..2^28 bytes, and B * C elements are at most 2^29 bytes; other strides take any value.  Outputs are contiguous [P][S][B][C].
  *   dtype: 0 f32, 1 bf16, 2 f16 - of every sequence, its gradient and the convolution's window; weights, their gradients and the scan's
  *   state are f32, and so is all arithmetic: a result is rounded once, when it is stored.
  *   weights are per network ([M][..][C]); net_of maps agents to networks as in marlhip_net_shape (n_networks == 0: one network an agent).
  *   reset u8 [S][B] or NULL: an episode starts at step t of row b - the state is zero before it, the window empty.
- *   lengths i32 [B] or NULL: steps of row b (clamped to 0..S).  Steps behind the end are not read; their outputs are 0 and the carried
- *   state is the one after the last step that counts.
- *   The carried state may be updated in place (h_out == h_in, state_out == state).
+ *   lengths i32 [B] or NULL: steps of row b (clamped to 0..S).  What stands in steps behind the end does not matter (it may be fetched, so the memory
+ *   has to be there); their outputs are 0 and the carried state is the one after the last step that counts.
+ *   The carried state may be updated in place (h_out == h_in, state_out == state); a gradient call then needs the state from before.  Other outputs
+ *   share no memory with inputs or with each other.
+ *   Arithmetic is f32's: outputs that an infinite or NaN input of their own episode reaches are not finite, infinite or NaN.
  *
- * Sums have a fixed order: equal inputs give equal bits.  Any S and B >= 0, C >= 1.
+ * Sums have a fixed order: equal inputs give equal bits.  0 <= S <= 2^30, 0 <= B <= 2^26, 1 <= C <= 2^20.
  * ---------------------------------------------------------------------------------------- */
 typedef struct marlhip_ssm_shape {
     int32_t n_agents, steps, batch, channels; /* P (1..16), S, B, C */
